@@ -6,5 +6,5 @@ Granite's backend / compute / operator interfaces (host/), and a thin ctypes
 mirror of that interface for tests and the benchmark.
 """
 from ._capi import GraniteHipError, LIB_PATH  # noqa: F401
-from .hip_compute import (DeviceBuffer, HipCompute, get_hip_compute, F16, F32, MASK_CAUSAL,  # noqa: F401
+from .hip_compute import (DeviceBuffer, HipCompute, get_hip_compute, F16, F32, F8E4M3, MASK_CAUSAL,  # noqa: F401
                           MASK_NONE, MASK_TREE, ROUND_NEAREST, ROUND_TRUNCATE)

@@ -14,7 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libgranite_hip.so"
 # constants of granite_hip.h
 OK = 0
 EINVAL, ENOTINIT, ENOMEM, EUNSUPPORTED, ENULL, EOVERFLOW, ESCRATCH = -1, -2, -3, -4, -5, -6, -7
-F32, F16 = 0, 1
+F32, F16, F8E4M3 = 0, 1, 2
 ROUND_TRUNCATE, ROUND_NEAREST = 0, 1
 MEM_DEVICE, MEM_SHARED, MEM_MANAGED = 0, 1, 2
 MASK_NONE, MASK_CAUSAL, MASK_TREE = 0, 1, 2
@@ -122,6 +122,47 @@ class RopeArgs(C.Structure):
     ]
 
 
+class KvForm(C.Structure):
+    _fields_ = [
+        ("kv_dtype", C.c_int),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("num_blocks", C.c_uint32),
+        ("window", C.c_uint32),
+        ("num_sinks", C.c_uint32),
+    ]
+
+
+class RopeQ8Args(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("src_dtype", C.c_int),
+        ("q_out_dtype", C.c_int),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("block_table", C.c_void_p),
+        ("cos_table", C.c_void_p),
+        ("sin_table", C.c_void_p),
+        ("table_positions", C.c_uint32),
+        ("freq_base", C.c_float),
+        ("num_heads_q", C.c_uint32),
+        ("num_heads_k", C.c_uint32),
+        ("seq_len", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("start_pos", C.c_uint32),
+        ("block_size", C.c_uint32),
+        ("num_blocks", C.c_uint32),
+        ("max_blocks_per_seq", C.c_uint32),
+        ("positions", C.c_void_p),
+        ("table_stride", C.c_int64),
+    ]
+
+
 _u32, _i64, _vp, _int, _f32 = C.c_uint32, C.c_int64, C.c_void_p, C.c_int, C.c_float
 
 # name -> (restype, argtypes); every symbol granite_hip.h declares
@@ -186,6 +227,13 @@ SIGNATURES = {
     "granite_hip_attention_workspace_required": (_int, [C.POINTER(AttentionArgs), C.POINTER(C.c_size_t)]),
     "granite_hip_decode_attention_ws": (_int, [C.POINTER(DecodeArgs), _vp, C.c_size_t]),
     "granite_hip_attention_ws": (_int, [C.POINTER(AttentionArgs), _vp, C.c_size_t]),
+    "granite_hip_decode_attention_ex": (_int, [C.POINTER(DecodeArgs), C.POINTER(KvForm), _vp, C.c_size_t]),
+    "granite_hip_attention_ex": (_int, [C.POINTER(AttentionArgs), C.POINTER(KvForm), _vp, C.c_size_t]),
+    "granite_hip_decode_ex_workspace_required": (
+        _int, [C.POINTER(DecodeArgs), C.POINTER(KvForm), C.POINTER(C.c_size_t)]),
+    "granite_hip_attention_ex_workspace_required": (
+        _int, [C.POINTER(AttentionArgs), C.POINTER(KvForm), C.POINTER(C.c_size_t)]),
+    "granite_hip_rope_append_q8": (_int, [C.POINTER(RopeQ8Args)]),
     "granite_hip_decode_attention_static": (_int, [C.POINTER(DecodeArgs)]),
     "granite_hip_static_scratch_bytes": (C.c_size_t, []),
 }

@@ -459,6 +459,47 @@ int granite_hip_attention_ws(const granite_hip_attention_args* args, void* works
     return ghip::launch_attention(*args, src);
 }
 
+// ---- 8-bit cache, sliding window: arguments are checked before the device is asked for ----
+
+int granite_hip_decode_attention_ex(const granite_hip_decode_args* args, const granite_hip_kv_form* form,
+                                    void* workspace, size_t workspace_bytes) {
+    if (!args || !form) return GRANITE_HIP_ENULL;
+    ghip::ScratchSource src;
+    src.fixed = workspace;
+    src.fixed_bytes = workspace_bytes;
+    return ghip::launch_decode_ex(*args, *form, src);
+}
+
+int granite_hip_attention_ex(const granite_hip_attention_args* args, const granite_hip_kv_form* form,
+                             void* workspace, size_t workspace_bytes) {
+    if (!args || !form) return GRANITE_HIP_ENULL;
+    ghip::ScratchSource src;
+    src.fixed = workspace;
+    src.fixed_bytes = workspace_bytes;
+    return ghip::launch_attention_ex(*args, *form, src);
+}
+
+int granite_hip_decode_ex_workspace_required(const granite_hip_decode_args* args, const granite_hip_kv_form* form,
+                                             size_t* bytes) {
+    if (!args || !form || !bytes) return GRANITE_HIP_ENULL;
+    ghip::ScratchSource src;
+    src.query = bytes;
+    return ghip::launch_decode_ex(*args, *form, src);
+}
+
+int granite_hip_attention_ex_workspace_required(const granite_hip_attention_args* args, const granite_hip_kv_form* form,
+                                                size_t* bytes) {
+    if (!args || !form || !bytes) return GRANITE_HIP_ENULL;
+    ghip::ScratchSource src;
+    src.query = bytes;
+    return ghip::launch_attention_ex(*args, *form, src);
+}
+
+int granite_hip_rope_append_q8(const granite_hip_rope_q8_args* args) {
+    if (!args) return GRANITE_HIP_ENULL;
+    return ghip::launch_rope_append_q8(*args);
+}
+
 int granite_hip_enable_kernel_timing(int enable) {
     GHIP_REQUIRE_INIT();
     ghip::resolve_timings();

@@ -1,0 +1,429 @@
+// Building blocks of the attention kernels over 8-bit pools and windowed caches (decode_ex.hip,
+// attention_ex.hip): the launch parameters and the work of one wave on one key tile.
+#pragma once
+
+#include "common.h"
+#include "kv_visible.h"
+
+namespace ghip {
+
+constexpr float kExLog2e = 1.4426950408889634f;
+constexpr float kExLn2 = 0.6931471805599453f;
+constexpr float kExNegBig = -1.0e30f;
+
+// How token positions map to rows.  Runs of 16 consecutive tokens that start at a multiple of 16 lie in
+// one block when the block size is a multiple of 16: one table entry, one scale and one base address
+// then serve 16 tokens and stay in scalar registers.
+enum : int { kExContiguous = 0, kExPaged16 = 1, kExPagedAny = 2 };
+
+struct KvParams {
+    const void* q;
+    int64_t q_batch, q_tok, q_head;  // element strides
+    const uint8_t* k;
+    const uint8_t* v;
+    const float* k_scale;  // 8-bit pools: [num_blocks, num_kv_heads]
+    const float* v_scale;
+    const int32_t* tables;
+    const int32_t* seq_lens;
+    void* out;
+    int64_t out_batch, out_tok, out_head;
+    float* lse;
+    int64_t lse_batch, lse_tok, lse_head;
+    float* part_o;  // split launches: unnormalised partial outputs
+    float* part_ml;
+    uint32_t* plan;
+    uint32_t batch, seq_q, num_heads, num_kv_heads, group;
+    uint32_t q_groups;  // runs of 16 query heads that share a KV head
+    uint32_t block_size, max_blocks, num_blocks;
+    int bs_shift;        // log2(block_size), -1 where it is no power of two
+    int64_t row_bytes;   // between consecutive rows of one KV head
+    int64_t head_bytes;  // between KV heads of one row
+    uint32_t max_tokens; // bound on any length
+    int decode;          // one query per sequence, at the sequence's last position
+    int causal;
+    int out_f32;
+    uint32_t start_pos, window, sinks;
+    uint32_t n_splits, q_tiles;
+    uint32_t workers, min_per, part_cap;
+    float scale_log2;
+};
+
+#if defined(__HIPCC__)
+
+__device__ __forceinline__ half8 ex_half8(uint4v x) { return __builtin_bit_cast(half8, x); }
+
+__device__ __forceinline__ uint32_t ex_lane_read(uint32_t v, uint32_t src_lane) {
+    return uint32_t(__builtin_amdgcn_ds_bpermute(int(src_lane << 2), int(v)));
+}
+__device__ __forceinline__ uint32_t ex_uniform(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_readfirstlane(int(v)));
+}
+
+// Two e4m3 codes (the low or the high half of `w`) as two halves.  Exact: a half holds every e4m3 value.
+template <bool kHigh>
+__device__ __forceinline__ uint32_t f8x2_to_f16x2(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(int(w), 1.0f, kHigh));
+}
+__device__ __forceinline__ half8 f8x8_to_half8(uint32_t a, uint32_t b) {
+    return ex_half8(uint4v{f8x2_to_f16x2<false>(a), f8x2_to_f16x2<true>(a), f8x2_to_f16x2<false>(b), f8x2_to_f16x2<true>(b)});
+}
+
+// Probabilities enter the second product times this: with V scales taken relative to the largest one
+// seen (ratios <= 1) a factor of 2^14 keeps the products of small ratios and probabilities in the normal range of
+// a half, 65504 being out of reach.
+constexpr float kExBoost = 16384.0f;
+
+__device__ __forceinline__ uint32_t ex_seq_len(const KvParams& p, uint32_t b) {
+    const uint32_t len = p.seq_lens ? uint32_t(max(p.seq_lens[b], 0)) : p.max_tokens;
+    return min(len, p.max_tokens);
+}
+
+// The work of one wave on one key tile, for up to 16 query rows (MFMA columns) of one KV head.
+//
+//   S^T[tok, row] = K[tok, :] . Q[row, :]     v_mfma_f32_16x16x32_f16 per 16 tokens and 32 elements
+//   softmax in the result layout: lane (n, g) holds row n, tokens 16 sub + 4 g + i
+//   O^T[d, row]  += V^T[d, tok] . P^T[tok, row]
+//
+// A tile is 64 tokens of an 8-bit cache or 32 of a half one: 64 registers of K and V per lane either
+// way.  K is the A operand as it lies in memory; the head-dim elements a lane holds for step s are
+// d_of(s, g) .. + 7, an order that only Q has to share: with 8 bits a lane reads a quarter of a row
+// in 16-byte pieces.  V^T takes the tokens of a step in the order 4 g + j, 16 + 4 g + j, which is how the first
+// product leaves the probabilities, and is put together from 4 x 4 byte (8 x 2 half) transposes with
+// v_perm_b32; row m of output tile t is d = 8 m + t, so a lane ends with 32 consecutive elements.
+// At head size 64 lanes 8 .. 15 of a group repeat the V loads of lanes 0 .. 7 and what they compute is dropped.
+template <bool kF8, int kRows, int kD>
+struct Tile {
+    static constexpr int kSubs = kF8 ? 4 : 2;
+    static constexpr uint32_t kTokens = 16 * kSubs;
+    static constexpr int kSteps = kD / 32;
+    static constexpr int kPairs = kSubs / 2;  // MFMA contractions (32 tokens) of the second product
+    static constexpr int kKLoads = kF8 ? kD / 64 : kSteps;
+    static constexpr int kVWords = kF8 ? 2 : 4;
+
+    static __device__ __forceinline__ uint32_t d_of(int s, uint32_t g) {
+        return kF8 ? (kD / 4) * g + 8 * s : 32 * s + 8 * g;
+    }
+
+    // Rows of a tile.  Paged16: lane l holds the row of token 16 (l & 3) of the tile (its 16-token
+    // run) and the run's scales; else: of token l & (kTokens - 1).
+    struct Rows {
+        uint32_t row;
+        float ks, vs;
+        uint32_t valid;
+    };
+    // tok0: first token of the tile.  `seen`: what the launch's or workgroup's queries see between
+    // them; the block table is not looked up beyond its end, and rows none of them sees have scale 0
+    // (whatever lies in the scale array there must not count as the largest).
+    // Whether some row that sees [lo, hi) and the sinks does not see some token of the tile, invalid pages
+    // included (uniform).
+    static __device__ __forceinline__ bool needs_mask(const KvParams& p, const Rows& r, uint32_t tok0, uint32_t lo, uint32_t hi) {
+        bool m = tok0 + kTokens > hi || (tok0 < lo && tok0 + kTokens > p.sinks);
+        if constexpr (kRows != kExContiguous) m = m || __any(r.valid == 0);
+        return m;
+    }
+
+    static __device__ __forceinline__ Rows rows_of(const KvParams& p, const int32_t* table, uint32_t kvh,
+                                                   uint32_t tok0, const VisibleTiles& seen, uint32_t lane) {
+        Rows r;
+        r.ks = r.vs = 1.0f;
+        r.valid = 1;
+        const uint32_t last = seen.end - 1;
+        if constexpr (kRows == kExContiguous) {
+            r.row = min(tok0 + (lane & (kTokens - 1)), last);
+        } else {
+            const uint32_t first = kRows == kExPaged16 ? tok0 + 16 * (lane & (kSubs - 1)) : tok0 + (lane & (kTokens - 1));
+            const uint32_t tok = min(first, last);
+            uint32_t blk, in;
+            if (p.bs_shift >= 0) {
+                blk = tok >> p.bs_shift;
+                in = tok & (p.block_size - 1);
+            } else {
+                blk = tok / p.block_size;
+                in = tok - blk * p.block_size;
+            }
+            // (a run whose first token is clamped to `last` keeps the clamped token's place in its
+            // 16-token run out of the row: the run is addressed from its start)
+            if constexpr (kRows == kExPaged16) in &= ~15u;
+            const int32_t entry = table[blk];
+            r.valid = pool_row(entry, in, p.block_size, p.num_blocks, &r.row) ? 1u : 0u;
+            if constexpr (kF8) {
+                const size_t at = size_t(r.valid ? uint32_t(entry) : 0u) * p.num_kv_heads + kvh;
+                const bool used = r.valid && first <= last &&
+                                  (first + (kRows == kExPaged16 ? 15 : 0) >= seen.lo || first < p.sinks);
+                const float ks = p.k_scale[at], vs = p.v_scale[at];
+                r.ks = used ? ks : 0.0f;
+                r.vs = used ? vs : 0.0f;
+            }
+        }
+        return r;
+    }
+
+    uint4v ka[kSubs][kKLoads];
+    uint32_t vr[kSubs * 4][kVWords];  // token 16 (j / 4) + 4 g + j % 4 at d = 8 n
+
+    __device__ __forceinline__ void load(const KvParams& p, const Rows& r, uint32_t kvh, uint32_t lane) {
+        const uint32_t n = lane & 15, g = lane >> 4;
+        const uint8_t* kb = p.k + int64_t(kvh) * p.head_bytes;
+        const uint8_t* vb = p.v + int64_t(kvh) * p.head_bytes;
+        constexpr uint32_t kElem = kF8 ? 1 : 2;
+        const uint32_t k_in = kElem * d_of(0, g), v_in = kElem * 8 * (n & (kD / 8 - 1));
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++) {
+            const uint8_t* kp;
+            if constexpr (kRows == kExPaged16) {
+                const uint32_t row = uint32_t(__builtin_amdgcn_readlane(int(r.row), sub));
+                kp = kb + uint64_t(row) * uint64_t(p.row_bytes) + (uint32_t(n) * uint32_t(p.row_bytes) + k_in);
+            } else {
+                kp = kb + uint64_t(ex_lane_read(r.row, 16 * sub + n)) * uint64_t(p.row_bytes) + k_in;
+            }
+#pragma unroll
+            for (int i = 0; i < kKLoads; i++)
+                ka[sub][i] = *reinterpret_cast<const uint4v*>(kp + (kF8 ? 16 : 64) * i);
+        }
+#pragma unroll
+        for (int j = 0; j < kSubs * 4; j++) {
+            const uint8_t* vp;
+            if constexpr (kRows == kExPaged16) {
+                const uint32_t row = uint32_t(__builtin_amdgcn_readlane(int(r.row), j / 4));
+                vp = vb + uint64_t(row) * uint64_t(p.row_bytes) + ((4 * g + j % 4) * uint32_t(p.row_bytes) + v_in);
+            } else {
+                vp = vb + uint64_t(ex_lane_read(r.row, 16 * (j / 4) + 4 * g + j % 4)) * uint64_t(p.row_bytes) + v_in;
+            }
+            // every byte of V is used once: streaming loads
+            if constexpr (kF8) {
+                const uint2v w = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(vp));
+                vr[j][0] = w.x;
+                vr[j][1] = w.y;
+            } else {
+                const uint4v w = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(vp));
+                vr[j][0] = w.x;
+                vr[j][1] = w.y;
+                vr[j][2] = w.z;
+                vr[j][3] = w.w;
+            }
+        }
+    }
+
+    // A operand of the first product: step s of sub-tile `sub`
+    __device__ __forceinline__ half8 k_operand(int sub, int s) const {
+        if constexpr (kF8) {
+            const uint4v w = ka[sub][s / 2];
+            return s % 2 ? f8x8_to_half8(w.z, w.w) : f8x8_to_half8(w.x, w.y);
+        } else {
+            return ex_half8(ka[sub][s]);
+        }
+    }
+    // A operands t = 4 w .. 4 w + 3 (8-bit) or 2 w, 2 w + 1 (half) of contraction `pair`
+    template <typename F>
+    __device__ __forceinline__ void v_operands(int pair, int w, F&& use) const {
+        const int j0 = 8 * pair;
+        if constexpr (kF8) {
+            // 4 x 4 byte transposes: tokens j0 .. j0 + 3 and j0 + 4 .. j0 + 7
+            uint32_t b[2][4];
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const uint32_t a0 = vr[j0 + 4 * q][w], a1 = vr[j0 + 4 * q + 1][w], a2 = vr[j0 + 4 * q + 2][w],
+                               a3 = vr[j0 + 4 * q + 3][w];
+                const uint32_t l01 = __builtin_amdgcn_perm(a1, a0, 0x05010400u);  // a0.0 a1.0 a0.1 a1.1
+                const uint32_t h01 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);  // a0.2 a1.2 a0.3 a1.3
+                const uint32_t l23 = __builtin_amdgcn_perm(a3, a2, 0x05010400u);
+                const uint32_t h23 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+                b[q][0] = __builtin_amdgcn_perm(l23, l01, 0x05040100u);
+                b[q][1] = __builtin_amdgcn_perm(l23, l01, 0x07060302u);
+                b[q][2] = __builtin_amdgcn_perm(h23, h01, 0x05040100u);
+                b[q][3] = __builtin_amdgcn_perm(h23, h01, 0x07060302u);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) use(4 * w + i, f8x8_to_half8(b[0][i], b[1][i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t sel = i ? 0x07060302u : 0x05040100u;
+                uint4v a;
+                a.x = __builtin_amdgcn_perm(vr[j0 + 1][w], vr[j0][w], sel);
+                a.y = __builtin_amdgcn_perm(vr[j0 + 3][w], vr[j0 + 2][w], sel);
+                a.z = __builtin_amdgcn_perm(vr[j0 + 5][w], vr[j0 + 4][w], sel);
+                a.w = __builtin_amdgcn_perm(vr[j0 + 7][w], vr[j0 + 6][w], sel);
+                use(2 * w + i, ex_half8(a));
+            }
+        }
+    }
+};
+
+// Query rows of a wave as B operands, and the running softmax state of those rows.  Float queries
+// are a half and a half remainder: nothing of them is lost.
+template <bool kQF32, bool kF8, int kD>
+struct Rows16 {
+    static constexpr int kSteps = kD / 32;
+    half8 bq[kSteps];
+    half8 bq_lo[kQF32 ? kSteps : 1];
+    float m, l;   // running maximum (log2 domain) and this lane's part of the sum
+    float vref, inv_vref;  // V scale the accumulators are relative to (from the start one whose inverse leaves room
+                           // for kExBoost: a tile of nothing but masked runs multiplies it by zero)
+    float4v acc[8];
+
+    __device__ __forceinline__ void clear() {
+        m = kExNegBig;
+        l = 0.0f;
+        vref = kF8 ? 0x1p-100f : 1.0f;
+        inv_vref = kF8 ? 0x1p+100f : 1.0f;
+#pragma unroll
+        for (int t = 0; t < 8; t++) acc[t] = float4v{0, 0, 0, 0};
+    }
+    // src: element offset of the lane's row; dead rows are zeros
+    __device__ __forceinline__ void load_q(const KvParams& p, int64_t at, bool live, uint32_t g) {
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+            const int64_t off = at + Tile<kF8, kExContiguous, kD>::d_of(s, g);
+            if constexpr (kQF32) {
+                const float* qp = static_cast<const float*>(p.q) + off;
+                const float4v x0 = *reinterpret_cast<const float4v*>(qp);
+                const float4v x1 = *reinterpret_cast<const float4v*>(qp + 4);
+                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                half8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float xv = live ? x[i] : 0.0f;
+                    const _Float16 h = static_cast<_Float16>(xv);
+                    hi[i] = h;
+                    lo[i] = static_cast<_Float16>(xv - static_cast<float>(h));
+                }
+                bq[s] = hi;
+                bq_lo[s] = lo;
+            } else {
+                uint4v w = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + off);
+                if (!live) w = uint4v{0, 0, 0, 0};
+                bq[s] = ex_half8(w);
+            }
+        }
+    }
+};
+
+// One tile's contribution to the rows of `st`.  `seen` is what all rows see between them, [lo, hi) and
+// the first `sinks` tokens what the lane's own row sees.  `masked` (uniform): some row does not see some
+// token of the tile.  kPerRow: the rows differ in what they see.
+//
+// V of a token that no row sees is zeroed, since 0 * NaN is NaN.  Where rows differ, a masked tile's V is
+// taken with its infinities and NaNs replaced by zeros, and two products with the indicators of
+// (+inf or NaN) and (-inf or NaN) in place of V and of visibility in place of P put them back into the
+// rows that do see them.
+template <bool kQF32, bool kF8, int kRows, int kD, bool kPerRow>
+__device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, kD>& tile,
+                                            const typename Tile<kF8, kRows, kD>::Rows& rows, uint32_t tok0,
+                                            const VisibleTiles& seen, uint32_t lo, uint32_t hi, bool masked,
+                                            Rows16<kQF32, kF8, kD>& st, uint32_t lane) {
+    using T = Tile<kF8, kRows, kD>;
+    constexpr int kSubs = T::kSubs;
+    const uint32_t g = lane >> 4;
+    // a value of the lane that holds token 16 sub + 4 g + i (Paged16: its run)
+    auto of_token = [&](float x, int sub, int i) __attribute__((always_inline)) -> float {
+        if constexpr (kRows == kExPaged16) return __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(__float_as_uint(x)), sub)));
+        else return __uint_as_float(ex_lane_read(__float_as_uint(x), 16 * sub + 4 * g + i));
+    };
+    float s[kSubs][4];
+#pragma unroll
+    for (int sub = 0; sub < kSubs; sub++) {
+        float4v c = {0, 0, 0, 0};
+#pragma unroll
+        for (int step = 0; step < T::kSteps; step++) {
+            const half8 a = tile.k_operand(sub, step);
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.bq[step], c, 0, 0, 0);
+            if constexpr (kQF32) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.bq_lo[step], c, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[sub][i] = c[i] * (kF8 ? of_token(rows.ks, sub, i) * p.scale_log2 : p.scale_log2);
+    }
+    uint32_t visible = 0xFFFFu;  // bit 4 sub + i: the lane's row sees token 16 sub + 4 g + i
+    if (masked) {
+        visible = 0;
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t in = 16 * sub + 4 * g + i, tok = tok0 + in;
+                const uint32_t valid = kRows == kExContiguous ? 1u
+                                       : kRows == kExPaged16  ? uint32_t(__builtin_amdgcn_readlane(int(rows.valid), sub))
+                                                              : ex_lane_read(rows.valid, in);
+                const bool vis = valid && tok < hi && (tok >= lo || tok < p.sinks);
+                if (vis) visible |= 1u << (4 * sub + i);
+                else s[sub][i] = -INFINITY;
+                const bool any = kPerRow ? valid && tok < seen.end && (tok >= seen.lo || tok < p.sinks) : vis;
+                if (!any) {
+#pragma unroll
+                    for (int w = 0; w < T::kVWords; w++) tile.vr[4 * sub + i][w] = 0;
+                }
+            }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 4 * kSubs; i++) top = fmaxf(top, s[i / 4][i % 4]);
+    top = fmaxf(top, wave_shfl_xor(top, 16));
+    top = fmaxf(top, wave_shfl_xor(top, 32));
+    const float m_new = fmaxf(st.m, top);
+    float rescale = fast_exp2(st.m - m_new);  // of O; of l without the change of the V scale
+    st.l *= rescale;
+    if constexpr (kF8) {
+        float vmax = rows.vs;
+        if constexpr (kRows == kExPaged16) {
+#pragma unroll
+            for (int sub = 0; sub < kSubs; sub++) vmax = fmaxf(vmax, of_token(rows.vs, sub, 0));
+        } else {
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) vmax = fmaxf(vmax, wave_shfl_xor(vmax, off));
+        }
+        if (__any(vmax > st.vref)) {  // the same in every lane
+            rescale *= st.vref / vmax;
+            st.vref = vmax;
+            st.inv_vref = 1.0f / vmax;
+        }
+    }
+    if (__any(m_new > st.m || rescale != 1.0f)) {
+#pragma unroll
+        for (int t = 0; t < 8; t++) st.acc[t] *= rescale;
+    }
+    st.m = m_new;
+    half8 hi8[T::kPairs], lo8[T::kPairs];
+#pragma unroll
+    for (int sub = 0; sub < kSubs; sub++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float e = fast_exp2(s[sub][i] - m_new);
+            st.l += e;
+            const float scaled = e * (kF8 ? of_token(rows.vs, sub, i) * (st.inv_vref * kExBoost) : kExBoost);
+            const _Float16 h = static_cast<_Float16>(scaled);
+            hi8[sub / 2][4 * (sub % 2) + i] = h;
+            lo8[sub / 2][4 * (sub % 2) + i] = static_cast<_Float16>(scaled - static_cast<float>(h));
+        }
+#pragma unroll
+    for (int pair = 0; pair < T::kPairs; pair++)
+#pragma unroll
+        for (int w = 0; w < T::kVWords; w++)
+            tile.v_operands(pair, w, [&](int t, half8 a) __attribute__((always_inline)) {
+                if (kPerRow && masked) {
+                    half8 plus, minus, sees;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const uint16_t bits = __builtin_bit_cast(uint16_t, _Float16(a[j]));
+                        const bool special = (bits & 0x7C00u) == 0x7C00u, nan = special && (bits & 0x3FFu);
+                        plus[j] = special && (nan || !(bits & 0x8000u)) ? _Float16(1) : _Float16(0);
+                        minus[j] = special && (nan || (bits & 0x8000u)) ? _Float16(1) : _Float16(0);
+                        if (special) a[j] = _Float16(0);
+                        sees[j] = (visible >> (8 * pair + j)) & 1u ? _Float16(1) : _Float16(0);
+                    }
+                    const float4v zero = {0, 0, 0, 0};
+                    const float4v up = __builtin_amdgcn_mfma_f32_16x16x32_f16(plus, sees, zero, 0, 0, 0);
+                    const float4v down = __builtin_amdgcn_mfma_f32_16x16x32_f16(minus, sees, zero, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (up[i] > 0.0f) st.acc[t][i] += INFINITY;
+                        if (down[i] > 0.0f) st.acc[t][i] -= INFINITY;
+                    }
+                }
+                st.acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi8[pair], st.acc[t], 0, 0, 0);
+                st.acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo8[pair], st.acc[t], 0, 0, 0);
+            });
+}
+
+#endif  // __HIPCC__
+
+}  // namespace ghip

@@ -13,8 +13,9 @@ from typing import Optional
 import numpy as np
 
 from . import _capi
-from ._capi import (F16, F32, MASK_CAUSAL, MASK_NONE, MASK_TREE, MEM_DEVICE, ROUND_NEAREST,
-                    ROUND_TRUNCATE, AttentionArgs, RopeArgs, DecodeArgs, check)
+from ._capi import (F16, F32, F8E4M3, MASK_CAUSAL, MASK_NONE, MASK_TREE, MEM_DEVICE, ROUND_NEAREST,
+                    ROUND_TRUNCATE, AttentionArgs, KvForm, RopeArgs, RopeQ8Args,
+                    DecodeArgs, check)
 
 
 class DeviceBuffer:
@@ -266,6 +267,66 @@ class HipCompute:
         else:
             check(self.lib.granite_hip_attention(C.byref(a)), "attention")
 
+    # ---- attention over 8-bit pools and through a sliding window with sinks
+    @staticmethod
+    def _workspace(workspace, workspace_bytes):
+        if workspace is None:
+            return None, 0
+        return _p(workspace), workspace.nbytes if workspace_bytes is None else workspace_bytes
+
+    def decode_attention_ex(self, *, q, q_dtype, k_cache, v_cache, out, batch_size, num_heads, num_kv_heads,
+                            head_dim, scale, kv_dtype, k_scale=None, v_scale=None, num_blocks=0, window=0,
+                            num_sinks=0, block_tables=None, seq_lens=None, lse=None, block_size=0,
+                            max_blocks_per_seq=0, max_seq=0, fixed_seq_len=0, workspace=None,
+                            workspace_bytes=None, query_workspace=False):
+        """decode_attention over a cache of kv_dtype (F8E4M3: paged, with k_scale / v_scale
+        [num_blocks, num_kv_heads]), each query seeing the last `window` tokens (0: all) and the
+        first num_sinks."""
+        a = DecodeArgs(_p(q), q_dtype, _p(k_cache), _p(v_cache), _p(block_tables), _p(seq_lens), _p(out), _p(lse),
+                       batch_size, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, max_seq,
+                       scale, fixed_seq_len, 0)
+        f = KvForm(kv_dtype, _p(k_scale), _p(v_scale), num_blocks, window, num_sinks)
+        if query_workspace:
+            need = C.c_size_t()
+            check(self.lib.granite_hip_decode_ex_workspace_required(C.byref(a), C.byref(f), C.byref(need)),
+                  "decode_ex_workspace_required")
+            return need.value
+        ws, ws_bytes = self._workspace(workspace, workspace_bytes)
+        check(self.lib.granite_hip_decode_attention_ex(C.byref(a), C.byref(f), ws, ws_bytes), "decode_attention_ex")
+
+    def attention_ex(self, *, q, q_dtype, q_tok_stride, q_head_stride, out, out_dtype, out_tok_stride,
+                     out_head_stride, seq_q, num_heads, num_kv_heads, head_dim, scale, k_cache, v_cache, cache_len,
+                     kv_dtype, k_scale=None, v_scale=None, num_blocks=0, window=0, num_sinks=0, max_seq=0,
+                     block_table=None, block_size=0, mask_mode=MASK_CAUSAL, start_pos=0, lse=None, workspace=None,
+                     workspace_bytes=None, query_workspace=False):
+        """attention over a cache of kv_dtype, with the window of decode_attention_ex at every query's
+        position start_pos + index."""
+        a = AttentionArgs(_p(q), q_dtype, q_tok_stride, q_head_stride, _p(out), out_dtype, out_tok_stride,
+                          out_head_stride, _p(lse), _p(k_cache), _p(v_cache), _p(block_table), block_size, max_seq,
+                          cache_len, None, None, 0, None, mask_mode, start_pos, seq_q, num_heads, num_kv_heads,
+                          head_dim, scale)
+        f = KvForm(kv_dtype, _p(k_scale), _p(v_scale), num_blocks, window, num_sinks)
+        if query_workspace:
+            need = C.c_size_t()
+            check(self.lib.granite_hip_attention_ex_workspace_required(C.byref(a), C.byref(f), C.byref(need)),
+                  "attention_ex_workspace_required")
+            return need.value
+        ws, ws_bytes = self._workspace(workspace, workspace_bytes)
+        check(self.lib.granite_hip_attention_ex(C.byref(a), C.byref(f), ws, ws_bytes), "attention_ex")
+
+    def rope_append_q8(self, *, seq_len, head_dim, src_dtype, q=None, q_out=None, q_out_dtype=F16, num_heads_q=0,
+                       k=None, v=None, num_heads_k=0, k_cache=None, v_cache=None, k_scale=None, v_scale=None,
+                       block_table=None, block_size=0, num_blocks=0, max_blocks_per_seq=0, start_pos=0,
+                       positions=None, table_stride=0, cos_table=None, sin_table=None, table_positions=0,
+                       freq_base=10000.0) -> None:
+        """rope_append into 8-bit pools with a scale per (block, KV head): Q rotated into q_out, K
+        (rotated) and V appended as e4m3 codes."""
+        a = RopeQ8Args(_p(q), _p(q_out), _p(k), _p(v), src_dtype, q_out_dtype, _p(k_cache), _p(v_cache), _p(k_scale),
+                       _p(v_scale), _p(block_table), _p(cos_table), _p(sin_table), table_positions, freq_base,
+                       num_heads_q, num_heads_k, seq_len, head_dim, start_pos, block_size, num_blocks,
+                       max_blocks_per_seq, _p(positions), table_stride)
+        check(self.lib.granite_hip_rope_append_q8(C.byref(a)), "rope_append_q8")
+
     # ---- scratch memory
     def workspace_bytes(self) -> int:
         return int(self.lib.granite_hip_workspace_bytes())
@@ -349,5 +410,5 @@ def get_hip_compute(device: int = 0) -> HipCompute:
     return _instance
 
 
-__all__ = ["DeviceBuffer", "HipCompute", "get_hip_compute", "F16", "F32", "MASK_CAUSAL",
+__all__ = ["DeviceBuffer", "HipCompute", "get_hip_compute", "F16", "F32", "F8E4M3", "MASK_CAUSAL",
            "MASK_NONE", "MASK_TREE", "ROUND_NEAREST", "ROUND_TRUNCATE"]

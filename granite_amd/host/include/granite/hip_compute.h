@@ -13,7 +13,9 @@
 
 struct granite_hip_attention_args;
 struct granite_hip_decode_args;
+struct granite_hip_kv_form;
 struct granite_hip_rope_args;
+struct granite_hip_rope_q8_args;
 
 namespace granite {
 
@@ -105,6 +107,20 @@ class HipCompute {
     // keys, causal / tree masks, optional log-sum-exp).
     Result<void> attention(const granite_hip_attention_args& args);
     Result<void> decode_attention(const granite_hip_decode_args& args);
+
+    // The same over 8-bit pools with block scales and through a sliding window with sinks
+    // (granite_hip_kv_form), and the rotation fused with the append to 8-bit pools.
+    // workspace NULL: the library's scratch.
+    Result<void> attention_ex(const granite_hip_attention_args& args, const granite_hip_kv_form& form,
+                              HipBuffer* workspace = nullptr, size_t workspace_bytes = 0);
+    Result<void> decode_attention_ex(const granite_hip_decode_args& args,
+                                     const granite_hip_kv_form& form,
+                                     HipBuffer* workspace = nullptr, size_t workspace_bytes = 0);
+    Result<size_t> attention_ex_workspace_required(const granite_hip_attention_args& args,
+                                                   const granite_hip_kv_form& form);
+    Result<size_t> decode_ex_workspace_required(const granite_hip_decode_args& args,
+                                                const granite_hip_kv_form& form);
+    Result<void> rope_append_q8(const granite_hip_rope_q8_args& args);
 
     // Scratch memory of the split-K launches.  MetalCompute's calls only enqueue
     // (src/backend/metal/metal_compute.mm:150-207); here a launch that needs more scratch

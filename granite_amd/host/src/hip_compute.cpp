@@ -208,6 +208,32 @@ Result<void> HipCompute::decode_attention_ws(const granite_hip_decode_args& args
     return HIP_CALL(granite_hip_decode_attention_ws(&args, workspace, workspace_bytes));
 }
 
+Result<void> HipCompute::attention_ex(const granite_hip_attention_args& args,
+                                      const granite_hip_kv_form& form, HipBuffer* workspace,
+                                      size_t workspace_bytes) {
+    return HIP_CALL(granite_hip_attention_ex(&args, &form, workspace, workspace_bytes));
+}
+Result<void> HipCompute::decode_attention_ex(const granite_hip_decode_args& args,
+                                             const granite_hip_kv_form& form, HipBuffer* workspace,
+                                             size_t workspace_bytes) {
+    return HIP_CALL(granite_hip_decode_attention_ex(&args, &form, workspace, workspace_bytes));
+}
+Result<size_t> HipCompute::attention_ex_workspace_required(const granite_hip_attention_args& args,
+                                                           const granite_hip_kv_form& form) {
+    size_t bytes = 0;
+    GRANITE_TRY(HIP_CALL(granite_hip_attention_ex_workspace_required(&args, &form, &bytes)));
+    return bytes;
+}
+Result<size_t> HipCompute::decode_ex_workspace_required(const granite_hip_decode_args& args,
+                                                        const granite_hip_kv_form& form) {
+    size_t bytes = 0;
+    GRANITE_TRY(HIP_CALL(granite_hip_decode_ex_workspace_required(&args, &form, &bytes)));
+    return bytes;
+}
+Result<void> HipCompute::rope_append_q8(const granite_hip_rope_q8_args& args) {
+    return HIP_CALL(granite_hip_rope_append_q8(&args));
+}
+
 HipCompute* get_hip_compute() {
     static HipCompute instance;
     static std::mutex guard;

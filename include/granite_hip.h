@@ -54,6 +54,8 @@ extern "C" {
 /* element types of Q / output tensors */
 #define GRANITE_HIP_F32 0
 #define GRANITE_HIP_F16 1
+/* element type of a key/value cache held in 8 bits (OCP e4m3, no infinities, largest value 448) */
+#define GRANITE_HIP_F8E4M3 2
 
 /* float -> half conversion used by the append entry points */
 #define GRANITE_HIP_ROUND_TRUNCATE 0 /* Granite's CPU fp32_to_fp16 (src/llm/math_ops.cpp:45-54) */
@@ -124,7 +126,8 @@ int granite_hip_event_elapsed_ms(void *start, void *stop, float *ms);
  * While enabled every launch is bracketed by two events on the launch stream.
  * Names: "kv_append", "kv_gather", "decode_stream" or "decode_splitk",
  * "decode_merge", "attention_tiles", "attention_merge", "tree_mask", "rope_append",
- * "matvec_q4k", "copy_rows".  granite_hip_kernel_timing_names() writes the
+ * "matvec_q4k", "copy_rows", "rope_append_q8", "decode_ex", "decode_ex_merge",
+ * "attention_ex", "attention_ex_merge".  granite_hip_kernel_timing_names() writes the
  * names seen so far, comma separated. */
 int granite_hip_enable_kernel_timing(int enable);
 int granite_hip_reset_kernel_timing(void);
@@ -456,6 +459,107 @@ size_t granite_hip_q4k_workspace_required(uint32_t K, uint64_t rows, uint32_t ba
 int granite_hip_matvec_q4k(const void *x, const void *w, void *y, uint32_t K, uint32_t N);
 int granite_hip_matvec_q4k_batched(const void *x, int64_t x_stride, const void *w, void *y,
                                    int64_t y_stride, uint32_t K, uint32_t N, uint32_t batch);
+
+/* ---- 8-bit key/value cache, sliding window with sinks -------------------- *
+ * The forms of the cache and of the mask that the entry points above do not have, over the
+ * same layouts.  The reference holds its cache in half precision and attends to all of it
+ * (src/llm/kv_cache.cpp:20-25, transformer.mm:1797-1806), so none of this has a counterpart
+ * there.
+ *
+ * 8-bit pools are paged pools [num_blocks*block_size, num_kv_heads, D] of e4m3 codes with one
+ * float scale for each (block, KV head) of K and of V, [num_blocks, num_kv_heads]: an element is
+ * code * scale.  granite_hip_rope_append_q8 writes scales that are powers of two (a power of two
+ * costs a floating-point code nothing, and a scale that grows later moves the codes of its block by
+ * whole exponents, which is exact down to code 2^-6); the attention entry points take any positive
+ * finite scale.
+ *
+ * Attention with these forms:
+ *   - a block-table entry outside [0, num_blocks) is never followed: its tokens count as not visible.
+ *     Under a window, entries of blocks that hold neither a token of the window nor a sink are not
+ *     used at all, so a caller can release those blocks and leave the entries stale;
+ *   - a query that sees no key (its window lies behind the cache, every page invalid) gets zeros and
+ *     a log-sum-exp of minus infinity;
+ *   - K or V values of tokens that a query does not see never reach its result, also where they are
+ *     NaN or infinite.
+ * Probabilities, sums and accumulators are float; decode and float outputs carry float precision
+ * (probabilities enter the second product as a half and a half remainder), half outputs take
+ * probabilities rounded to half. */
+typedef struct granite_hip_kv_form {
+    int kv_dtype;         /* GRANITE_HIP_F16 or GRANITE_HIP_F8E4M3 (paged pools only) */
+    const float *k_scale; /* F8E4M3: float[num_blocks, num_kv_heads] */
+    const float *v_scale;
+    uint32_t num_blocks;  /* paged: blocks the pools hold */
+    uint32_t window;      /* a query at position p sees keys p-window+1 .. p; 0: no window */
+    uint32_t num_sinks;   /* ... and the first num_sinks keys (no meaning without a window) */
+} granite_hip_kv_form;
+
+/* granite_hip_decode_attention over a cache of the given form.  The query of a sequence of length n
+ * is at position n - 1.  chunk_tokens is not used.  workspace / workspace_bytes as in
+ * granite_hip_decode_attention_ws; workspace NULL: the library's buffer.  Half pools without a window
+ * are handed to granite_hip_decode_attention (which takes block tables as they are). */
+int granite_hip_decode_attention_ex(const granite_hip_decode_args *args,
+                                    const granite_hip_kv_form *form, void *workspace,
+                                    size_t workspace_bytes);
+/* granite_hip_attention over a cache of the given form; mask_mode CAUSAL (query q is at position
+ * start_pos + q), or NONE without a window.  Trees and extra keys: GRANITE_HIP_EUNSUPPORTED.  Half
+ * caches without a window are handed to granite_hip_attention. */
+int granite_hip_attention_ex(const granite_hip_attention_args *args,
+                             const granite_hip_kv_form *form, void *workspace,
+                             size_t workspace_bytes);
+/* Scratch bytes the launch needs, as granite_hip_decode_workspace_required. */
+int granite_hip_decode_ex_workspace_required(const granite_hip_decode_args *args,
+                                             const granite_hip_kv_form *form, size_t *bytes);
+int granite_hip_attention_ex_workspace_required(const granite_hip_attention_args *args,
+                                                const granite_hip_kv_form *form, size_t *bytes);
+
+/* granite_hip_rope_append into 8-bit pools: rotates Q and K and appends K and V, one launch.
+ *   q             [seq_len, num_heads_q, D] of src_dtype, NULL: none; q_out receives it rotated,
+ *                 same layout, F32 or F16 (round to nearest).  q_out may be q itself where both
+ *                 types are F32
+ *   k, v          [seq_len, num_heads_k, D] of src_dtype, read only; NULL (both): only Q
+ *   src_dtype     GRANITE_HIP_F32 or GRANITE_HIP_F16, of q, k and v
+ *   cos/sin       as in granite_hip_rope_append: with tables the rotation is RoPECache::apply's
+ *                 bit for bit (every product and sum rounded to float), without them it is
+ *                 evaluated from freq_base
+ *   k_cache ...   8-bit pools and their scales, as above; block_table as in granite_hip_rope_append
+ *   positions     NULL: one sequence, tokens start_pos .. start_pos + seq_len - 1 through one
+ *                 block table of max_blocks_per_seq entries.  Else device int32[seq_len], one token
+ *                 of seq_len different sequences: token s goes to position positions[s] through
+ *                 block_table + s * table_stride (table_stride >= max_blocks_per_seq when
+ *                 seq_len > 1).  Different sequences append to different blocks: a block that two
+ *                 tables share is not written to.
+ * The scale of a block and head covers the tokens appended to it since its first row was last
+ * written: a call that writes row 0 of a block starts it anew, any other keeps the larger of
+ * the old scale and the one the new rows need, and where that grows rounds the rows in front
+ * of the new ones to it.  The scale the new rows need is the smallest power of two s, 2^-96 <= s <=
+ * 2^120, with every finite new element of the block and head at most 448 s; codes are rounded to
+ * nearest even, infinities become +-448 s, NaN stays NaN.  Rows behind the new ones are left as they
+ * were.  A token whose position is negative, beyond the cos/sin tables or whose block-table
+ * entry is outside [0, num_blocks) is not stored (the first two also leave its q_out row as it
+ * was). */
+typedef struct granite_hip_rope_q8_args {
+    const void *q;
+    void *q_out;
+    const void *k;
+    const void *v;
+    int src_dtype;
+    int q_out_dtype;
+    void *k_cache;
+    void *v_cache;
+    float *k_scale;
+    float *v_scale;
+    const int32_t *block_table;
+    const float *cos_table;
+    const float *sin_table;
+    uint32_t table_positions;
+    float freq_base;
+    uint32_t num_heads_q, num_heads_k, seq_len, head_dim, start_pos;
+    uint32_t block_size, num_blocks, max_blocks_per_seq;
+    const int32_t *positions;
+    int64_t table_stride;
+} granite_hip_rope_q8_args;
+
+int granite_hip_rope_append_q8(const granite_hip_rope_q8_args *args);
 
 /* ---- scratch memory ------------------------------------------------------ *
  * Decode and prefill launches that split the keys over several workgroups
