@@ -1,0 +1,817 @@
+// Attention of a run of queries over 8-bit paged pools, and through a sliding window with sinks: the tiles
+// kernel for gfx950 and the merge of its key splits.
+//
+// What it computes is written at granite_hip_attention_ex (granite_hip.h).  The arithmetic is that of
+// attention_tiles_kernel (prefill.hip): S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16, a wave owning 32
+// query rows, K and V tiles of 64 keys in LDS as halves, a three-stage pipeline over 32-key sub-tiles (scores of
+// j + 1, softmax of j, second product of j - 1 in one phase, vector work spread behind the MFMAs).  What is new:
+//
+// * Rows are (query, head of the KV head's group) pairs, row = query * group + head, so a workgroup's 256 rows
+//   share one KV head's tiles and cover few positions: 256 / group of them.  Under a window a workgroup visits
+//   window + 256 / group keys for rows that see `window` each (with a head to itself it would visit window + 256), and
+//   a chunk of 37 queries in groups of 4 is one workgroup's worth of rows instead of four quarter-full ones.
+// * Codes become halves once per workgroup, on the way from registers to LDS (v_cvt_scalef32_pk_f16_fp8,
+//   two a cycle and lane): a half holds every e4m3 value, so the products are those of the codes themselves.  Converting
+//   operands as they are read would put four conversions beside every MFMA of every wave.
+// * Scales never touch an element of K or V.  A run of 16 keys lies in one block (block sizes are multiples of
+//   16 here), so a sub-tile has two scales of K and two of V.  K's goes into the factor that takes a score to the
+//   log2 domain.  V's enters the exponent: with x = score + log2(v scale) the probabilities p' = exp2(x - ref)
+//   carry it, the second product takes the codes, and the sum l takes each run's p' times 1 / (v scale).  The
+//   reference follows x, so a large or small V scale never pushes p' out of the range of a half.  Cost per sub-tile:
+//   two subtractions and one more multiply-add than without scales.
+// * Tiles are visited by the list of kv_visible.h: those of the sinks, then those of the window.
+//
+// Probabilities are rounded to half; with float outputs (kPrecise) they are a half and a half remainder and the
+// second product runs twice.  Sums and accumulators are float.
+//
+// V of keys that no row of the workgroup sees is stored as zeros, since 0 * NaN is NaN.  In tiles that only
+// some rows see, infinities and NaNs of V are stored as zeros as well, and where there were any they are added
+// at the end to the rows that see them (add_specials).
+#include "common.h"
+#include "kv_attend.h"
+
+namespace ghip {
+namespace {
+
+constexpr int kBM = 256;  // query rows per workgroup
+constexpr int kBN = 64;   // keys per tile
+constexpr int kThreads = 512;
+constexpr int kKBuffers = 3, kVBuffers = 3;
+constexpr float kProbLimit = 16384.0f;  // a row's probabilities of a sub-tile may sum to this much
+
+template <int kD>
+struct Shape {
+    static constexpr int kKPitch = kD + 8;  // halves
+    static constexpr int kVPitch = kD;      // halves, 64-byte chunks swizzled with the key
+    static constexpr int kKTile = kBN * kKPitch, kVTile = kBN * kVPitch;
+    static constexpr size_t kTileBytes = size_t(kKBuffers * kKTile + kVBuffers * kVTile) * sizeof(uint16_t);
+    static constexpr size_t kLdsBytes = kTileBytes + kKBuffers * 4 * sizeof(float4v) + 16;
+    static constexpr int kSteps = kD / 16;   // MFMAs of the scores of a sub-tile
+    static constexpr int kBlocks = kD / 32;  // 32-row head-dim blocks of O^T
+    static constexpr int kPhase = kSteps + 2 * kBlocks;
+};
+
+// Halves of x that are infinite or NaN become zero; whether there were any.
+__device__ __forceinline__ bool drop_specials(uint4v& x) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool lo = (x[i] & 0x7C00u) == 0x7C00u, hi = (x[i] & 0x7C000000u) == 0x7C000000u;
+        if (lo) x[i] &= 0xFFFF0000u;
+        if (hi) x[i] &= 0x0000FFFFu;
+        any = any || lo || hi;
+    }
+    return any;
+}
+
+template <bool kQF32, bool kPrecise, bool kF8, int kRows, int kD>
+__global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
+    using S = Shape<kD>;
+    constexpr int kKPitch = S::kKPitch, kVPitch = S::kVPitch, kKTile = S::kKTile, kVTile = S::kVTile, kSteps = S::kSteps,
+                  kBlocks = S::kBlocks, kPhase = S::kPhase;
+    extern __shared__ __attribute__((aligned(16))) uint16_t s_mem[];
+    uint16_t* const s_k0 = s_mem;
+    uint16_t* const s_v0 = s_mem + kKBuffers * kKTile;
+    // of run i of the tile in K buffer b: scale of the scores, log2 of the V scale, its inverse, valid
+    float4v* const s_run = reinterpret_cast<float4v*>(reinterpret_cast<unsigned char*>(s_mem) + S::kTileBytes);
+    uint32_t* const s_special = reinterpret_cast<uint32_t*>(s_run + kKBuffers * 4);
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = ex_uniform(tid >> 6);
+    const uint32_t n = lane & 31, g = lane >> 5;
+
+    // ---- which (KV head, key split, row tile): ids are handed to the 8 XCDs round-robin, so they are remapped
+    // for the workgroups that stream the same keys to share an L2
+    uint32_t job = blockIdx.x;
+    {
+        constexpr uint32_t kXcds = 8;
+        if (gridDim.x % kXcds == 0) job = (job % kXcds) * (gridDim.x / kXcds) + job / kXcds;
+    }
+    const uint32_t slot = job % p.q_tiles, rest = job / p.q_tiles;
+    const uint32_t split = rest % p.n_splits, kvh = rest / p.n_splits;
+
+    // ---- rows.  Two runs of 128, four waves each, one wave of each on a SIMD.  Where the keys a row sees grow with
+    // its position (causal, no window, few keys in front), the k-th run from the end is paired with the k-th from
+    // the start, so that every workgroup has the same work (p.paired, set by the launcher).
+    constexpr uint32_t kHalf = kBM / 2;
+    const uint32_t n_rows = p.seq_q * p.group;
+    const uint32_t halves = (n_rows + kHalf - 1) / kHalf;
+    const uint32_t late_half = p.paired ? halves - 1 - slot : 2 * slot + 1;
+    const uint32_t early_half = p.paired ? slot : 2 * slot;
+    const bool second_run = wave >= kThreads / 128;
+    const bool run_live = !second_run || early_half < late_half;
+    const uint32_t my_half = (p.paired != 0) == second_run ? early_half : late_half;
+    const uint32_t r0 = run_live ? my_half * kHalf + 32 * (wave & 3) : n_rows;
+    const bool wave_active = r0 < n_rows;
+    const uint32_t row = min(r0 + n, n_rows - 1);
+    const bool row_live = r0 + n < n_rows;
+    const uint32_t query = row / p.group, head = kvh * p.group + (row - query * p.group);
+
+    // ---- keys: of the workgroup, of this wave, of this lane's row
+    auto pos_of = [&](uint32_t r) __attribute__((always_inline)) { return p.start_pos + min(r, n_rows - 1) / p.group; };
+    const uint32_t wg_first = pos_of(early_half * kHalf), wg_last = pos_of((late_half + 1) * kHalf - 1);
+    const uint32_t len = p.max_tokens;
+    auto limit_of = [&](uint32_t pos) __attribute__((always_inline)) { return p.causal ? min(len, pos + 1) : len; };
+    const VisibleTiles seen = visible_tiles<kBN>(wg_first, limit_of(wg_last), p.window, p.sinks);
+    const uint32_t all_hi = limit_of(wg_first), all_lo = window_begin(wg_last, p.window);  // seen by every row
+    const uint32_t t_begin = uint32_t(uint64_t(seen.count) * split / p.n_splits);
+    const uint32_t n_tiles = uint32_t(uint64_t(seen.count) * (split + 1) / p.n_splits);
+    // keys from `cap` on belong to the next split: the tile that a wave may compute beyond its share is masked whole
+    const uint32_t cap = n_tiles < seen.count ? seen.tile(n_tiles) * kBN : 0xFFFFFFFFu;
+    const uint32_t wave_first = pos_of(r0), wave_last = pos_of(r0 + 31);
+    const uint32_t wave_hi = limit_of(wave_last);  // behind the last key any row of the wave sees
+    const uint32_t every_hi = min(limit_of(wave_first), cap), every_lo = window_begin(wave_last, p.window);  // every row sees
+    const uint32_t row_hi = min(limit_of(p.start_pos + query), cap), row_lo = window_begin(p.start_pos + query, p.window);
+
+    // ---- Q^T as B operand: lane (n, g), step s holds Q[row][16 s + 8 g .. + 7]
+    half8 bq[kSteps];
+    half8 bq_lo[kQF32 ? kSteps : 1];
+    {
+        const int64_t off = int64_t(query) * p.q_tok + int64_t(head) * p.q_head + 8 * g;
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+            if constexpr (kQF32) {
+                const float* qp = static_cast<const float*>(p.q) + off + 16 * s;
+                const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
+                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                half8 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float xs = x[i] * p.q_sign;
+                    const _Float16 h = static_cast<_Float16>(xs);
+                    hi[i] = h;
+                    lo[i] = static_cast<_Float16>(xs - static_cast<float>(h));
+                }
+                bq[s] = hi;
+                bq_lo[s] = lo;
+            } else {
+                bq[s] = ex_half8(*reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + off + 16 * s)) * _Float16(p.q_sign);
+            }
+        }
+    }
+
+    float m_ref = kExNegBig, l_run = 0.0f;
+    float16v oacc[kBlocks];
+#pragma unroll
+    for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) oacc[t][r] = 0.0f;
+
+    // ---- staging: a thread moves a piece of key ld_r of K and of V; the eight threads of a key cover its row.
+    // The keys of a wave's pieces (8 of them) lie in one run.
+    const uint32_t ld_c = tid & 7, ld_r = tid >> 3;
+    constexpr uint32_t kPieceHalves = kD / 8;                 // per thread and row
+    constexpr bool kTwo = kD == 128;                          // two 16-byte stores
+    constexpr uint32_t kRegs = (kF8 ? kD / 8 : kD / 4) / 4;   // registers of a piece as loaded: 2, 4 or 8
+    constexpr uint32_t kSwz = kBlocks - 1;
+    // 8 bits: 16 (8) consecutive elements from kPieceHalves * ld_c on.  Half: 8 from 8 ld_c on and, of 128, 8 from 64 on.
+    const uint32_t e0 = kF8 ? kPieceHalves * ld_c : 8 * ld_c, e1 = kF8 ? e0 + 8 : e0 + 64;
+    auto v_at = [&](uint32_t e) __attribute__((always_inline)) { return ld_r * kVPitch + ((((e >> 5) ^ (ld_r & kSwz)) << 5) | (e & 31)); };
+    const uint32_t k_st0 = ld_r * kKPitch + e0, k_st1 = ld_r * kKPitch + e1, v_st0 = v_at(e0), v_st1 = v_at(e1);
+    const uint8_t* const k_base = p.k + int64_t(kvh) * p.head_bytes + (kF8 ? e0 : 2 * e0);
+    const uint8_t* const v_base = p.v + int64_t(kvh) * p.head_bytes + (kF8 ? e0 : 2 * e0);
+
+    // The 8 keys of a wave's pieces lie in one run of 16, so the block-table entry, the address of their first row and
+    // their scales are the wave's; a lane adds its row's and column's offset.
+    const uint32_t wave_key = 8 * wave;
+    const uint32_t lane_off = (ld_r & 7) * uint32_t(p.row_bytes);
+    auto key_of = [&](uint32_t it) __attribute__((always_inline)) { return seen.tile(it) * kBN; };  // first key of the it-th tile
+    auto staged = [&](uint32_t it) __attribute__((always_inline)) { return key_of(min(it, n_tiles - 1)); };
+    struct Place {
+        uint32_t blk, in;  // block-table index and row in the block of the wave's first key
+    };
+    auto place_of = [&](uint32_t it) __attribute__((always_inline)) -> Place {
+        const uint32_t key = min(staged(it) + wave_key, (seen.end - 1) & ~7u);
+        Place r;
+        if (p.bs_shift >= 0) {
+            r.blk = key >> p.bs_shift;
+            r.in = key & (p.block_size - 1);
+        } else {
+            r.blk = key / p.block_size;
+            r.in = key - r.blk * p.block_size;
+        }
+        return r;
+    };
+    auto lookup = [&](uint32_t it) __attribute__((always_inline)) -> int32_t {  // the entry, one value for the wave
+        if constexpr (kRows == kExContiguous) return 0;
+        else return p.tables[place_of(it).blk];
+    };
+    struct Piece {
+        uint32_t k[kRegs], v[kRegs];
+        float ks, vs;  // of the run of its K
+    };
+    auto fetch = [&](uint32_t (&dst)[kRegs], const uint8_t* src) __attribute__((always_inline)) {
+        if constexpr (kRegs == 2) {
+            const uint2v w = *reinterpret_cast<const uint2v*>(src);
+            dst[0] = w.x;
+            dst[1] = w.y;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kRegs / 4; i++) {
+                const uint4v w = *reinterpret_cast<const uint4v*>(src + 128 * i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) dst[4 * i + j] = w[j];
+            }
+        }
+    };
+    // Row of the wave's first key of tile `it` (its validity in `valid`), from its table entry.
+    struct RowAt {
+        uint32_t row, valid;
+    };
+    auto row_at = [&](uint32_t it, int32_t entry) __attribute__((always_inline)) -> RowAt {
+        RowAt r;
+        r.valid = 1;
+        if constexpr (kRows == kExContiguous) {
+            r.row = staged(it);
+        } else {
+            r.valid = pool_row(int32_t(ex_uniform(uint32_t(entry))), place_of(it).in, p.block_size, p.num_blocks, &r.row) ? 1u : 0u;
+        }
+        return r;
+    };
+    auto piece_at = [&](const uint8_t* base, const RowAt& r) __attribute__((always_inline)) -> const uint8_t* {
+        if constexpr (kRows == kExContiguous) {
+            // (rows behind the last key may lie behind the cache's end: the last one instead)
+            return base + uint64_t(min(r.row + ld_r, len - 1)) * uint64_t(p.row_bytes);
+        } else {
+            return base + uint64_t(r.row) * uint64_t(p.row_bytes) + lane_off;
+        }
+    };
+    auto load_k = [&](const RowAt& r, int32_t entry, Piece& piece) __attribute__((always_inline)) {
+        if constexpr (kF8) {
+            const uint64_t sc = uint64_t(r.valid ? ex_uniform(uint32_t(entry)) : 0u) * p.num_kv_heads + kvh;
+            piece.ks = p.k_scale[sc];
+            piece.vs = p.v_scale[sc];
+        }
+        fetch(piece.k, piece_at(k_base, r));
+    };
+    auto load_v = [&](const RowAt& r, Piece& piece) __attribute__((always_inline)) { fetch(piece.v, piece_at(v_base, r)); };
+    auto halves_of = [&](const uint32_t (&src)[kRegs], int half) __attribute__((always_inline)) -> uint4v {
+        if constexpr (kF8) {
+            return __builtin_bit_cast(uint4v, f8x8_to_half8(src[2 * half], src[2 * half + 1]));
+        } else {
+            return uint4v{src[4 * half], src[4 * half + 1], src[4 * half + 2], src[4 * half + 3]};
+        }
+    };
+    auto store_k = [&](uint32_t buf, uint32_t valid, const Piece& piece) __attribute__((always_inline)) {
+        uint16_t* s = s_k0 + buf * kKTile;
+        *reinterpret_cast<uint4v*>(s + k_st0) = halves_of(piece.k, 0);
+        if constexpr (kTwo) *reinterpret_cast<uint4v*>(s + k_st1) = halves_of(piece.k, 1);
+        if (kRows != kExContiguous && (tid & 127) == 0) {  // one thread per run
+            // (a run that nobody sees may have anything for scales; a masked score, minus infinity, must come
+            // through the factor and the shift as what it is: a positive factor, a finite shift)
+            const float vs = kF8 && valid ? fminf(fmaxf(piece.vs, 0x1p-100f), 0x1p+126f) : 1.0f;
+            float4v info;
+            info.x = kF8 && valid ? fmaxf(fmaxf(piece.ks, 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
+            info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
+            info.z = 1.0f / vs;
+            info.w = valid ? 1.0f : 0.0f;
+            s_run[buf * 4 + (tid >> 7)] = info;
+        }
+    };
+    // Whether some row of the workgroup does not see some key of the tile that begins at key0.
+    auto partial = [&](uint32_t key0) __attribute__((always_inline)) {
+        return key0 + kBN > all_hi || (key0 < all_lo && key0 + kBN > p.sinks);
+    };
+    auto store_v = [&](uint32_t buf, uint32_t it, uint32_t valid, const Piece& piece) __attribute__((always_inline)) {
+        uint16_t* s = s_v0 + buf * kVTile;
+        uint4v x0 = halves_of(piece.v, 0), x1 = {0, 0, 0, 0};
+        if constexpr (kTwo) x1 = halves_of(piece.v, 1);
+        const uint32_t key0 = staged(it);
+        if (partial(key0) || (kRows != kExContiguous && !valid)) {
+            const uint32_t key = key0 + ld_r;
+            bool special = drop_specials(x0);
+            if constexpr (kTwo) special = drop_specials(x1) || special;
+            if (!valid || key >= seen.end || (key < seen.lo && key >= p.sinks)) {
+                x0 = x1 = uint4v{0, 0, 0, 0};
+                special = false;
+            }
+            if (special) *s_special = 1;
+        }
+        *reinterpret_cast<uint4v*>(s + v_st0) = x0;
+        if constexpr (kTwo) *reinterpret_cast<uint4v*>(s + v_st1) = x1;
+    };
+
+    // ---- V^T operand reads through ds_read_b64_tr_b16 (see prefill.hip): 16-lane group q4, lane 4 k4 + r4 of it points
+    // at key 4 g + k4, head-dim elements 32 t + 16 (q4 & 1) + 8 (r4 & 1) + 4 (r4 >> 1) .. + 3
+    uint32_t vt_off[kBlocks];
+    {
+        const uint32_t q4 = lane >> 4, i16 = lane & 15, k4 = i16 >> 2, r4 = i16 & 3, key = 4 * g + k4;
+        const uint32_t in_chunk = 16 * (q4 & 1) + 8 * (r4 & 1) + 4 * (r4 >> 1);
+#pragma unroll
+        for (uint32_t t = 0; t < uint32_t(kBlocks); t++) vt_off[t] = key * kVPitch + (((t ^ (k4 & kSwz)) << 5) | in_chunk);
+    }
+    auto v_pair = [&](const uint16_t* vp) __attribute__((always_inline)) -> half8 {
+        const uint2v lo = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4v __attribute__((address_space(3)))*)(vp)));
+        const uint2v hi = __builtin_bit_cast(uint2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4v __attribute__((address_space(3)))*)(vp + 8 * kVPitch)));
+        return ex_half8(uint4v{lo.x, lo.y, hi.x, hi.y});
+    };
+
+    // ---- per-tile pieces of a wave
+    struct Run {
+        float scale, lvs, inv;
+    };
+    struct Runs {
+        Run r[2];
+        bool valid;  // both
+        uint32_t bits;
+    };
+    auto runs_of = [&](uint32_t kbuf, int sub) __attribute__((always_inline)) -> Runs {
+        Runs x;
+        x.bits = 3;
+        if constexpr (kRows == kExContiguous) {
+            x.r[0] = x.r[1] = Run{p.scale_log2, 0.0f, 1.0f};
+        } else {
+            const float4v a = s_run[kbuf * 4 + 2 * sub], b = s_run[kbuf * 4 + 2 * sub + 1];
+            x.bits = ex_uniform((a.w != 0.0f ? 1u : 0u) | (b.w != 0.0f ? 2u : 0u));
+            if constexpr (kF8) {
+                x.r[0] = Run{a.x, a.y, a.z};
+                x.r[1] = Run{b.x, b.y, b.z};
+            } else {
+                x.r[0] = x.r[1] = Run{p.scale_log2, 0.0f, 1.0f};
+            }
+        }
+        x.valid = x.bits == 3;
+        return x;
+    };
+    // keys of the sub-tile at key0 that the lane's row does not see become minus infinity
+    auto apply_mask = [&](uint32_t key0, uint32_t bits, float16v& s) __attribute__((always_inline)) {
+        if (key0 + 32 <= every_hi && (key0 >= every_lo || key0 + 32 <= p.sinks) && bits == 3) return;
+        // what depends on the lane goes into three numbers, the rest is a constant per element; no short-circuit logic,
+        // so that it stays compares and selects
+        const int32_t base = int32_t(key0 + 4 * g), lo = int32_t(row_lo) - base, sink = int32_t(p.sinks) - base;
+        const int32_t hi[2] = {bits & 1u ? int32_t(row_hi) - base : -1, bits & 2u ? int32_t(row_hi) - base : -1};
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int32_t in = 8 * (r >> 2) + (r & 3);
+            const bool vis = bool(int(in < hi[r >> 3]) & (int(in >= lo) | int(in < sink)));
+            s[r] = vis ? s[r] : -INFINITY;
+        }
+    };
+    auto scores = [&](uint32_t kbuf, int sub, float16v& out) __attribute__((always_inline)) {
+        const uint16_t* krow = s_k0 + kbuf * kKTile + (32 * sub + n) * kKPitch + 8 * g;
+        float16v c = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+            const half8 a = ex_half8(*reinterpret_cast<const uint4v*>(krow + 16 * s));
+            c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bq[s], c, 0, 0, 0);
+            if constexpr (kQF32) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bq_lo[s], c, 0, 0, 0);
+        }
+        out = c;
+    };
+    struct Probs {
+        half8 hi[2];
+        half8 lo[kPrecise ? 2 : 1];
+    };
+    // Probabilities are relative to a reference that moves only when those of a sub-tile sum to kProbLimit or more
+    // (or to infinity, as in the first), see prefill.hip.
+    auto rebase = [&](const float16v& s, const Runs& runs) __attribute__((always_inline)) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; r++) top = fmaxf(top, __builtin_fmaf(s[r], runs.r[r >> 3].scale, runs.r[r >> 3].lvs));
+        const LanePair both = half_wave_pair(top);
+        const float m_new = fmaxf(m_ref, fmaxf(both.lo, both.hi));
+        const float alpha = fast_exp2(m_ref - m_new);
+        m_ref = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) oacc[t][r] *= alpha;
+    };
+    auto pack = [&](const float* pe, half8& hi, half8* lo) __attribute__((always_inline)) {  // 8 probabilities
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const _Float16 h = static_cast<_Float16>(pe[j]);
+            hi[j] = h;
+            if constexpr (kPrecise) (*lo)[j] = static_cast<_Float16>(pe[j] - static_cast<float>(h));
+        }
+    };
+    auto probabilities_once = [&](const float16v& s, const Runs& runs, Probs& out, float (&sum)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const float shift = runs.r[u].lvs - m_ref;
+            float pe[8];
+            sum[u] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                pe[j] = fast_exp2(__builtin_fmaf(s[8 * u + j], runs.r[u].scale, shift));
+                sum[u] += pe[j];
+            }
+            pack(pe, out.hi[u], &out.lo[kPrecise ? u : 0]);
+        }
+    };
+    auto probabilities = [&](const float16v& s, const Runs& runs, Probs& out) __attribute__((always_inline)) {
+        float sum[2];
+        probabilities_once(s, runs, out, sum);
+        if (__any(!(sum[0] + sum[1] < kProbLimit))) {
+            rebase(s, runs);
+            probabilities_once(s, runs, out, sum);
+        }
+        l_run += sum[0] * runs.r[0].inv + sum[1] * runs.r[1].inv;
+    };
+    auto accumulate = [&](uint32_t vbuf, int sub, const Probs& pr) __attribute__((always_inline)) {
+        const uint16_t* sv = s_v0 + vbuf * kVTile + 32 * sub * kVPitch;
+#pragma unroll
+        for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const half8 a = v_pair(sv + vt_off[t] + 16 * u * kVPitch);
+                oacc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pr.hi[u], oacc[t], 0, 0, 0);
+                if constexpr (kPrecise) oacc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pr.lo[u], oacc[t], 0, 0, 0);
+            }
+    };
+    // One phase of the pipeline: scores of sub-tile j + 1 (key0_q, buffer kbuf), softmax of j (s_in, runs_in), second
+    // product of j - 1.  `side(step)` is the caller's work in the shadow of the MFMAs.
+    auto fused_phase = [&](uint32_t key0_q, uint32_t kbuf, int sub_q, float16v& s_out, const float16v& s_in, const Runs& runs_in,
+                           Probs& p_out, uint32_t vbuf, int sub_v, const Probs& p_prev, auto&& side) __attribute__((always_inline)) {
+        const uint16_t* krow = s_k0 + kbuf * kKTile + (32 * sub_q + n) * kKPitch + 8 * g;
+        const uint16_t* sv = s_v0 + vbuf * kVTile + 32 * sub_v * kVPitch;
+        auto k_operand = [&](int s) __attribute__((always_inline)) { return ex_half8(*reinterpret_cast<const uint4v*>(krow + 16 * s)); };
+        auto v_operand = [&](int i) __attribute__((always_inline)) { return v_pair(sv + vt_off[i % kBlocks] + 16 * (i / kBlocks) * kVPitch); };
+        constexpr int kRing = 3;
+        half8 ring[kRing];
+#pragma unroll
+        for (int i = 0; i < kRing - 1; i++) ring[i] = k_operand(i);
+        float16v c = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        const float shift[2] = {runs_in.r[0].lvs - m_ref, runs_in.r[1].lvs - m_ref};
+        float psum[2] = {0.0f, 0.0f};
+        float pe[16];
+        uint32_t pw[8], pl[kPrecise ? 8 : 1];
+        float tn = __builtin_fmaf(s_in[0], runs_in.r[0].scale, shift[0]);
+        auto finish = [&](int i) __attribute__((always_inline)) {  // elements 2 i, 2 i + 1
+            pw[i] = pack_f16x2(pe[2 * i], pe[2 * i + 1]);
+            if constexpr (kPrecise) {
+                const half2v h = __builtin_bit_cast(half2v, pw[i]);
+                pl[i] = pack_f16x2(pe[2 * i] - static_cast<float>(h.x), pe[2 * i + 1] - static_cast<float>(h.y));
+                asm volatile("" : "+v"(pl[i]));
+            }
+            asm volatile("" : "+v"(pw[i]));
+        };
+        auto softmax_step = [&](int e) __attribute__((always_inline)) {
+            pe[e] = fast_exp2(tn);
+            if (e < 15) tn = __builtin_fmaf(s_in[e + 1], runs_in.r[(e + 1) >> 3].scale, shift[(e + 1) >> 3]);
+            if (e > 0) psum[(e - 1) >> 3] += pe[e - 1];
+            if (e > 0 && (e & 1) == 0) finish(e / 2 - 1);
+            asm volatile("" : "+v"(pe[e]), "+v"(tn), "+v"(psum[0]), "+v"(psum[1]));
+        };
+        constexpr int kPer = 16 / kPhase;
+        auto vector_work = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < kPer; j++) softmax_step(step * kPer + j);
+            side(step);
+        };
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+            if (s + kRing - 1 < kSteps) ring[(s + kRing - 1) % kRing] = k_operand(s + kRing - 1);
+            c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[s % kRing], bq[s], c, 0, 0, 0);
+            if constexpr (kQF32) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[s % kRing], bq_lo[s], c, 0, 0, 0);
+            vector_work(s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < kRing - 1; i++) ring[i] = v_operand(i);
+        apply_mask(key0_q, kRows == kExContiguous ? 3u : runs_of(kbuf, sub_q).bits, c);  // rare
+#pragma unroll
+        for (int i = 0; i < 2 * kBlocks; i++) {
+            if (i + kRing - 1 < 2 * kBlocks) ring[(i + kRing - 1) % kRing] = v_operand(i + kRing - 1);
+            oacc[i % kBlocks] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], p_prev.hi[i / kBlocks], oacc[i % kBlocks], 0, 0, 0);
+            if constexpr (kPrecise)
+                oacc[i % kBlocks] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % kRing], p_prev.lo[i / kBlocks], oacc[i % kBlocks], 0, 0, 0);
+            vector_work(kSteps + i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        psum[1] += pe[15];
+        finish(7);
+        p_out.hi[0] = ex_half8(uint4v{pw[0], pw[1], pw[2], pw[3]});
+        p_out.hi[1] = ex_half8(uint4v{pw[4], pw[5], pw[6], pw[7]});
+        if constexpr (kPrecise) {
+            p_out.lo[0] = ex_half8(uint4v{pl[0], pl[1], pl[2], pl[3]});
+            p_out.lo[1] = ex_half8(uint4v{pl[4], pl[5], pl[6], pl[7]});
+        }
+        if (__any(!(psum[0] + psum[1] < kProbLimit))) {  // rare: the reference has to move, redo the sub-tile
+            rebase(s_in, runs_in);
+            probabilities_once(s_in, runs_in, p_out, psum);
+        }
+        l_run += psum[0] * runs_in.r[0].inv + psum[1] * runs_in.r[1].inv;
+        s_out = c;
+    };
+
+    if (tid == 0) *s_special = 0;
+    __syncthreads();
+    if (t_begin < n_tiles) {  // uniform; an empty share writes a neutral partial
+        // Tiles this wave computes: up to the last one that holds a key some row of it sees, in pairs (a tile that
+        // is one too many, or in front of a later window's first, is masked whole).  There is one code path: both
+        // phases run in every iteration, and where a stage does not apply yet it works on zero probabilities.
+        uint32_t my_end = t_begin;
+        if (wave_active)
+            for (uint32_t it = n_tiles; it > t_begin; it--)
+                if (key_of(it - 1) < wave_hi) {
+                    my_end = it;
+                    break;
+                }
+        my_end += (my_end - t_begin) & 1;
+
+        // ---- prologue: in LDS K of the first two tiles and V of the first, in flight K of the third and fourth and V of
+        // the second and third, lookups two tiles further
+        Piece a, b;
+        const int32_t e0_ = lookup(t_begin), e1_ = lookup(t_begin + 1), e2_ = lookup(t_begin + 2), e3_ = lookup(t_begin + 3);
+        const RowAt o0 = row_at(t_begin, e0_), o1 = row_at(t_begin + 1, e1_), o2 = row_at(t_begin + 2, e2_), o3 = row_at(t_begin + 3, e3_);
+        load_k(o0, e0_, a);
+        load_v(o0, a);
+        load_k(o1, e1_, b);
+        store_k(0, o0.valid, a);
+        store_v(0, t_begin, o0.valid, a);
+        store_k(1, o1.valid, b);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(o2, e2_, a);
+        load_v(o1, a);
+        __builtin_amdgcn_sched_barrier(0);
+        int32_t look_a = lookup(t_begin + 4);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(o3, e3_, b);
+        load_v(o2, b);
+        __builtin_amdgcn_sched_barrier(0);
+        int32_t look_b = lookup(t_begin + 5);
+        __builtin_amdgcn_sched_barrier(0);
+        RowAt at_v = o3;  // of the tile whose V is loaded next
+        // validity of the tiles in flight: K of it + 2 and it + 3, V of it + 1 and it + 2 (bit 0 the nearer)
+        uint32_t k_valid = o2.valid | (o3.valid << 1), v_valid = o1.valid | (o2.valid << 1);
+        __syncthreads();
+
+        float16v s0, s1;
+        Probs p_old, p_new;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            p_old.hi[u] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+            if constexpr (kPrecise) p_old.lo[u] = p_old.hi[u];
+        }
+        if (my_end > t_begin) {
+            scores(0, 0, s0);
+            apply_mask(key_of(t_begin), runs_of(0, 0).bits, s0);
+        }
+        uint32_t kb_cur = 0, kb_next = 1, kb_store = 2;
+        // (the first iteration's second product, of nothing, reads the first tile's V: whatever it holds, every row sees it)
+        uint32_t vb_prev = 0, vb_cur = 0, vb_store = 1;
+        auto staging = [&](uint32_t it, Piece& piece, int32_t& look, int part) __attribute__((always_inline)) {
+            if (part == 0) store_k(kb_store, k_valid & 1, piece);           // K of tile it + 2
+            if (part == 2) store_v(vb_store, it + 1, v_valid & 1, piece);   // V of tile it + 1
+            if (part == 4) {
+                const RowAt at_k = row_at(it + 4, look);  // K of it + 4, V of it + 3
+                load_k(at_k, look, piece);
+                load_v(at_v, piece);
+                k_valid = (k_valid >> 1) | (at_k.valid << 1);
+                v_valid = (v_valid >> 1) | (at_v.valid << 1);
+                at_v = at_k;
+            }
+            if (part == 5) look = lookup(it + 6);
+        };
+        auto rotate_buffers = [&]() __attribute__((always_inline)) {
+            __syncthreads();
+            const uint32_t kf = kb_cur;
+            kb_cur = kb_next;
+            kb_next = kb_store;
+            kb_store = kf;
+            vb_prev = vb_cur;
+            vb_cur = vb_store;
+            vb_store = 3 - vb_prev - vb_cur;
+        };
+        auto iteration = [&](uint32_t it, Piece& piece, int32_t& look) __attribute__((always_inline)) {
+            const uint32_t key_cur = key_of(it), key_nxt = key_of(it + 1);
+            const Runs ra = runs_of(kb_cur, 0);
+            fused_phase(key_cur + 32, kb_cur, 1, s1, s0, ra, p_new, vb_prev, 1, p_old, [&](int step) { staging(it, piece, look, step - (kPhase - 8)); });
+            const Runs rb = runs_of(kb_cur, 1);
+            fused_phase(key_nxt, kb_next, 0, s0, s1, rb, p_old, vb_cur, 0, p_new, [](int) {});
+            rotate_buffers();
+        };
+        auto stage_only = [&](uint32_t it, Piece& piece, int32_t& look) __attribute__((always_inline)) {
+#pragma unroll
+            for (int part = 0; part < 6; part++) staging(it, piece, look, part);
+            rotate_buffers();
+        };
+        uint32_t it = t_begin;
+        for (; it < my_end; it += 2) {
+            iteration(it, a, look_a);
+            iteration(it + 1, b, look_b);
+        }
+        if (my_end > t_begin) accumulate(vb_prev, 1, p_old);
+        for (; it < n_tiles; it += 2) {
+            stage_only(it, a, look_a);
+            stage_only(it + 1, b, look_b);
+        }
+    }
+
+    if (!wave_active) return;
+    {
+        const LanePair both = half_wave_pair(l_run);
+        l_run = both.lo + both.hi;
+    }
+    if (!row_live) return;
+    // Accumulator [t][4 a + b] is head-dim element 32 t + 16 (a >> 1) + 8 g + 4 (a & 1) + b: 8 consecutive per (t, a >> 1).
+    if (t_begin < n_tiles && *s_special) {
+        // infinities and NaNs of V that were left out in tiles that not every row sees (rare)
+        for (uint32_t it = t_begin; it < n_tiles; it++) {
+            const uint32_t key0 = key_of(it);
+            if (!partial(key0)) continue;
+            for (uint32_t key = key0; key < min(key0 + kBN, row_hi); key++) {
+                if (key < row_lo && key >= p.sinks) continue;
+                uint32_t at = key;
+                if constexpr (kRows != kExContiguous) {
+                    const uint32_t blk = key / p.block_size;
+                    if (!pool_row(p.tables[blk], key - blk * p.block_size, p.block_size, p.num_blocks, &at)) continue;
+                }
+                const uint8_t* v = p.v + int64_t(kvh) * p.head_bytes + int64_t(at) * p.row_bytes;
+#pragma unroll
+                for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const uint32_t d = 32 * t + 16 * (r >> 3) + 8 * g + (r & 7);
+                        if constexpr (kF8) {
+                            if ((v[d] & 0x7Fu) == 0x7Fu) oacc[t][r] = NAN;
+                        } else {
+                            const float x = static_cast<float>(reinterpret_cast<const _Float16*>(v)[d]);
+                            if (!(fabsf(x) < INFINITY)) oacc[t][r] += x;
+                        }
+                    }
+            }
+        }
+    }
+    if (p.n_splits > 1) {
+        const size_t at = (size_t(split) * p.num_kv_heads + kvh) * n_rows + row;
+        float* po = p.part_o + at * kD;
+#pragma unroll
+        for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+            for (int ah = 0; ah < 2; ah++) {
+                float* op = po + 32 * t + 16 * ah + 8 * g;
+                *reinterpret_cast<float4v*>(op) = float4v{oacc[t][8 * ah], oacc[t][8 * ah + 1], oacc[t][8 * ah + 2], oacc[t][8 * ah + 3]};
+                *reinterpret_cast<float4v*>(op + 4) = float4v{oacc[t][8 * ah + 4], oacc[t][8 * ah + 5], oacc[t][8 * ah + 6], oacc[t][8 * ah + 7]};
+            }
+        if (g == 0) {
+            p.part_ml[at * 2] = m_ref;
+            p.part_ml[at * 2 + 1] = l_run;
+        }
+        return;
+    }
+    const bool none = l_run == 0.0f;  // the row sees no key
+    const float inv_l = none ? 0.0f : 1.0f / l_run;
+    const int64_t off = int64_t(query) * p.out_tok + int64_t(head) * p.out_head;
+#pragma unroll
+    for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+        for (int ah = 0; ah < 2; ah++) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = oacc[t][8 * ah + e] * inv_l;
+            const uint32_t d = 32 * t + 16 * ah + 8 * g;
+            if constexpr (kPrecise) {
+                float* op = static_cast<float*>(p.out) + off + d;
+                *reinterpret_cast<float4v*>(op) = float4v{x[0], x[1], x[2], x[3]};
+                *reinterpret_cast<float4v*>(op + 4) = float4v{x[4], x[5], x[6], x[7]};
+            } else {
+                uint4v w;
+                w.x = pack_f16x2(x[0], x[1]);
+                w.y = pack_f16x2(x[2], x[3]);
+                w.z = pack_f16x2(x[4], x[5]);
+                w.w = pack_f16x2(x[6], x[7]);
+                *reinterpret_cast<uint4v*>(static_cast<uint16_t*>(p.out) + off + d) = w;
+            }
+        }
+    if (p.lse && g == 0)
+        p.lse[int64_t(head) * p.lse_head + query] = none ? -INFINITY : (m_ref + __builtin_amdgcn_logf(l_run)) * kExLn2;
+}
+
+// Joins the key splits of 2048 / D rows of one KV head: a thread per eight head-dim elements.
+template <bool kOutF32, int kD>
+__global__ void __launch_bounds__(256) kv_tiles_merge_kernel(KvParams p) {
+    constexpr uint32_t kLanes = kD / 8;
+    const uint32_t n_rows = p.seq_q * p.group, kvh = blockIdx.y;
+    const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes, dc = threadIdx.x % kLanes;
+    if (row >= n_rows) return;
+    float mx = kExNegBig, l = 0.0f;
+    float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (uint32_t s0 = 0; s0 < p.n_splits; s0 += 4) {  // four at a time: their loads are in flight together
+        float m[4], ls[4];
+        float4v a[4], b[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const size_t at = (size_t(min(s0 + i, p.n_splits - 1)) * p.num_kv_heads + kvh) * n_rows + row;
+            m[i] = p.part_ml[at * 2];
+            ls[i] = p.part_ml[at * 2 + 1];
+            a[i] = *reinterpret_cast<const float4v*>(p.part_o + at * kD + 8 * dc);
+            b[i] = *reinterpret_cast<const float4v*>(p.part_o + at * kD + 8 * dc + 4);
+        }
+        float m_new = mx;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) m_new = fmaxf(m_new, s0 + i < p.n_splits ? m[i] : kExNegBig);
+        const float keep = fast_exp2(mx - m_new);
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] *= keep;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            if (s0 + i >= p.n_splits) continue;
+            const float f = fast_exp2(m[i] - m_new);
+            l += ls[i] * f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                o[e] += a[i][e] * f;
+                o[4 + e] += b[i][e] * f;
+            }
+        }
+        mx = m_new;
+    }
+    const bool none = l == 0.0f;
+    const float inv_l = none ? 0.0f : 1.0f / l;
+    const uint32_t query = row / p.group, head = kvh * p.group + row % p.group;
+    const int64_t off = int64_t(query) * p.out_tok + int64_t(head) * p.out_head + 8 * dc;
+    if constexpr (kOutF32) {
+        float* op = static_cast<float*>(p.out) + off;
+        *reinterpret_cast<float4v*>(op) = float4v{o[0] * inv_l, o[1] * inv_l, o[2] * inv_l, o[3] * inv_l};
+        *reinterpret_cast<float4v*>(op + 4) = float4v{o[4] * inv_l, o[5] * inv_l, o[6] * inv_l, o[7] * inv_l};
+    } else {
+        uint4v w;
+        w.x = pack_f16x2(o[0] * inv_l, o[1] * inv_l);
+        w.y = pack_f16x2(o[2] * inv_l, o[3] * inv_l);
+        w.z = pack_f16x2(o[4] * inv_l, o[5] * inv_l);
+        w.w = pack_f16x2(o[6] * inv_l, o[7] * inv_l);
+        *reinterpret_cast<uint4v*>(static_cast<uint16_t*>(p.out) + off) = w;
+    }
+    if (p.lse && dc == 0) p.lse[int64_t(head) * p.lse_head + query] = none ? -INFINITY : (mx + __builtin_amdgcn_logf(l)) * kExLn2;
+}
+
+template <bool kQF32, bool kPrecise, bool kF8, int kRows, int kD>
+int launch_one(const KvParams& p, dim3 grid) {
+    auto kernel = kv_tiles_kernel<kQF32, kPrecise, kF8, kRows, kD>;
+    static bool configured[kMaxDevices];
+    if (int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(kernel), Shape<kD>::kLdsBytes, configured)) return rc;
+    kernel<<<grid, dim3(kThreads), Shape<kD>::kLdsBytes, ctx().stream>>>(p);
+    return launch_status();
+}
+template <bool kQF32, bool kPrecise, int kD>
+int launch_cache(const KvParams& p, dim3 grid, bool f8, int rows) {
+    if (f8) return launch_one<kQF32, kPrecise, true, kExPaged16, kD>(p, grid);
+    if (rows == kExPaged16) return launch_one<kQF32, kPrecise, false, kExPaged16, kD>(p, grid);
+    return launch_one<kQF32, kPrecise, false, kExContiguous, kD>(p, grid);
+}
+template <int kD>
+int launch_types(const KvParams& p, dim3 grid, bool q_f32, bool f8, int rows) {
+    if (q_f32 && p.out_f32) return launch_cache<true, true, kD>(p, grid, f8, rows);
+    if (q_f32) return launch_cache<true, false, kD>(p, grid, f8, rows);
+    if (p.out_f32) return launch_cache<false, true, kD>(p, grid, f8, rows);
+    return launch_cache<false, false, kD>(p, grid, f8, rows);
+}
+
+}  // namespace
+
+int launch_kv_tiles(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const ScratchSource& scratch) {
+    const uint64_t n_rows = uint64_t(p.seq_q) * p.group;
+    if (n_rows >= (1ull << 31)) return GRANITE_HIP_EINVAL;
+    p.q_tiles = uint32_t((n_rows + kBM - 1) / kBM);
+    // With a window every row sees about as many keys, and behind a long prefix nearly as many.
+    p.paired = p.causal && p.window == 0 && p.start_pos < 4 * uint64_t(p.seq_q);
+    // the factor of the scores is positive in the kernel (see the runs' scales there): a negative one's sign, and the
+    // zero of a zero one, go to Q
+    p.q_sign = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
+    p.scale_log2 = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
+    const uint32_t cus = ctx().compute_units > 0 ? uint32_t(ctx().compute_units) : 256u;
+    const uint64_t wgs = uint64_t(p.q_tiles) * p.num_kv_heads;
+    // tiles of a workgroup: the window's, those its rows' positions add to it, the sinks'
+    const uint64_t keys = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + kBM / p.group) : p.max_tokens;
+    const uint32_t tiles = uint32_t((keys + kBN - 1) / kBN);
+    p.n_splits = 1;
+    if (wgs < cus) p.n_splits = min(min(uint32_t((cus + wgs - 1) / wgs), max(tiles / 4, 1u)), 64u);
+    const size_t slots = p.n_splits > 1 ? size_t(p.n_splits) * p.num_kv_heads * n_rows : 0;
+    const size_t need = slots * (D + 2) * sizeof(float);
+    if (scratch.query) {
+        *scratch.query = need;
+        return GRANITE_HIP_OK;
+    }
+    if (wgs * p.n_splits > 0x7FFFFFFFull || p.num_kv_heads > 65535u) return GRANITE_HIP_EINVAL;
+    if (need > 0) {
+        void* ws = nullptr;
+        if (int rc = take_scratch(scratch, need, &ws)) return rc;
+        p.part_o = static_cast<float*>(ws);
+        p.part_ml = p.part_o + slots * D;
+    }
+    int rc;
+    {
+        KernelTimerScope timer("attention_ex");
+        const dim3 grid(uint32_t(wgs * p.n_splits));
+        rc = D == 128 ? launch_types<128>(p, grid, q_f32, f8, rows) : launch_types<64>(p, grid, q_f32, f8, rows);
+    }
+    if (rc != GRANITE_HIP_OK || p.n_splits == 1) return rc;
+    {
+        KernelTimerScope timer("attention_ex_merge");
+        const dim3 grid(uint32_t((n_rows + 2048 / D - 1) / (2048 / D)), p.num_kv_heads), block(256);
+        hipStream_t st = ctx().stream;
+        if (D == 128) {
+            if (p.out_f32) kv_tiles_merge_kernel<true, 128><<<grid, block, 0, st>>>(p);
+            else kv_tiles_merge_kernel<false, 128><<<grid, block, 0, st>>>(p);
+        } else {
+            if (p.out_f32) kv_tiles_merge_kernel<true, 64><<<grid, block, 0, st>>>(p);
+            else kv_tiles_merge_kernel<false, 64><<<grid, block, 0, st>>>(p);
+        }
+    }
+    return launch_status();
+}
+
+}  // namespace ghip

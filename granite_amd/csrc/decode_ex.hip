@@ -210,7 +210,7 @@ int check_form(const granite_hip_kv_form& f, const void* k, const void* v, const
     p.block_size = table ? block_size : 1;
     p.bs_shift = (p.block_size & (p.block_size - 1)) == 0 ? __builtin_ctz(p.block_size) : -1;
     p.window = f.window;
-    p.sinks = f.window ? f.num_sinks : 0;
+    p.sinks = f.window ? min(f.num_sinks, 0x7FFFFFFFu) : 0;
     return GRANITE_HIP_OK;
 }
 
@@ -323,6 +323,8 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     p.causal = a.mask_mode == GRANITE_HIP_MASK_CAUSAL;
     p.start_pos = a.start_pos;
     p.scale_log2 = a.scale * kExLog2e;
+    if (rows != kExPagedAny && uint64_t(a.seq_q) * p.group > 32)
+        return launch_kv_tiles(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
     return launch_rows(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
 }
 

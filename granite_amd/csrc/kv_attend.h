@@ -44,9 +44,14 @@ struct KvParams {
     int out_f32;
     uint32_t start_pos, window, sinks;
     uint32_t n_splits, q_tiles;
+    uint32_t paired;     // tiles kernel: late and early runs of rows share a workgroup
     uint32_t workers, min_per, part_cap;
     float scale_log2;
+    float q_sign;  // tiles kernel: 1, -1 or 0, taken into Q
 };
+
+// attention_ex.hip: the tiles kernel.  Block sizes are multiples of 16, or the cache is contiguous.
+int launch_kv_tiles(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const ScratchSource& scratch);
 
 #if defined(__HIPCC__)
 
@@ -344,10 +349,10 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
                 const uint32_t valid = kRows == kExContiguous ? 1u
                                        : kRows == kExPaged16  ? uint32_t(__builtin_amdgcn_readlane(int(rows.valid), sub))
                                                               : ex_lane_read(rows.valid, in);
-                const bool vis = valid && tok < hi && (tok >= lo || tok < p.sinks);
+                const bool vis = bool(int(valid) & int(tok < hi) & (int(tok >= lo) | int(tok < p.sinks)));
                 if (vis) visible |= 1u << (4 * sub + i);
                 else s[sub][i] = -INFINITY;
-                const bool any = kPerRow ? valid && tok < seen.end && (tok >= seen.lo || tok < p.sinks) : vis;
+                const bool any = kPerRow ? bool(int(valid) & int(tok < seen.end) & (int(tok >= seen.lo) | int(tok < p.sinks))) : vis;
                 if (!any) {
 #pragma unroll
                     for (int w = 0; w < T::kVWords; w++) tile.vr[4 * sub + i][w] = 0;

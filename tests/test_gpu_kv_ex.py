@@ -116,8 +116,9 @@ def run_decode(gpu, cache, hq, q_dtype, window=0, sinks=0, lens=None, seed=0, wh
 
 
 def run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype, window=0, sinks=0, cache_len=None, seed=0, heads_first=False,
-                mask=MASK_CAUSAL, what="prefill", **more):
+                mask=MASK_CAUSAL, what="prefill", scale=None, **more):
     d = cache.d
+    scale = d ** -0.5 if scale is None else scale
     length = cache.lens[0] if cache_len is None else cache_len
     rng = np.random.default_rng(seed + 7)
     q = rng.standard_normal((n, hq, d)).astype(np.float16 if q_dtype == F16 else np.float32)
@@ -126,7 +127,7 @@ def run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype, window=0, sinks=0,
     strides = (d, n * d) if heads_first else (hq * d, d)
     out, lse, dq = dev(np.full(stored.shape, 7.0, odt)), dev(np.full((hq, n), 7.0, np.float32)), dev(stored)
     gpu.attention_ex(q=dq, q_dtype=q_dtype, q_tok_stride=strides[0], q_head_stride=strides[1], out=out, out_dtype=out_dtype,
-                     out_tok_stride=strides[0], out_head_stride=strides[1], seq_q=n, num_heads=hq, scale=d ** -0.5,
+                     out_tok_stride=strides[0], out_head_stride=strides[1], seq_q=n, num_heads=hq, scale=scale,
                      cache_len=length, block_table=cache.dev[4], mask_mode=mask, start_pos=start, lse=lse, window=window,
                      num_sinks=sinks, **cache.kwargs(), **more)
     gpu.sync()
@@ -134,7 +135,7 @@ def run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype, window=0, sinks=0,
     got = got.transpose(1, 0, 2) if heads_first else got
     (k, v), valid = cache.rows(0, length)
     vis = kv8.visible(start + np.arange(n), length, window, sinks, valid, mask == MASK_CAUSAL)
-    o, l, ds = kv8.attend(q, k, v, vis, d ** -0.5)
+    o, l, ds = kv8.attend(q, k, v, vis, scale)
     check(got, lse.read(np.float32, (hq, n)).T, o, l, ds, v_top(v, vis), int(vis.sum(1).max()), out_dtype == F16, what)
     return got
 
@@ -330,6 +331,23 @@ def test_prefill_scales(gpu):
             for bs in (16, 20):
                 run_prefill(gpu, Cache(np.random.default_rng(9), [700], bs, 2, 128, F8E4M3, spread=spread, scales=scales).upload(), 180, 520,
                             4, F16, out, what=f"scales {scales} {spread}")
+
+
+@pytest.mark.parametrize("out_dtype", [F16, F32])
+@pytest.mark.parametrize("scale", [20.0, -0.3, 0.0, 1e-30])
+def test_prefill_other_factors(gpu, out_dtype, scale):
+    for kv, bs in ((F8E4M3, 16), (F16, 16), (F16, 0)):
+        cache = Cache(np.random.default_rng(20), [400], bs, 2, 64, kv).upload()
+        run_prefill(gpu, cache, 150, 250, 4, F32, out_dtype, window=120, sinks=3, scale=scale, what=f"scale {scale}")
+
+
+@pytest.mark.parametrize("n,start,hq,hkv", [(9, 20000, 8, 1), (40, 9000, 4, 2), (300, 5000, 2, 1), (64, 3333, 8, 2)])
+def test_prefill_keys_split(gpu, n, start, hq, hkv):
+    """Few rows over many keys: the keys are cut into several parts, with odd numbers of tiles in them."""
+    for q, o in ((F16, F16), (F32, F32)):
+        cache = Cache(np.random.default_rng(n), [start + n], 16, hkv, 128, F8E4M3).upload()
+        run_prefill(gpu, cache, n, start, hq, q, o)
+        run_prefill(gpu, cache, n, start, hq, q, o, window=2345, sinks=70)
 
 
 # ------------------------------------------------------------------ both
