@@ -9,6 +9,7 @@ namespace ghip {
 namespace {
 
 constexpr uint32_t kRowWaves = 4;
+constexpr uint32_t kDirectTiles = 12;
 
 // One workgroup per (run of 16 query rows, KV head, sequence, key split).  A row is a (query, head of
 // the KV head's group) pair, row r = query * group + head, so a decode step's group, a few draft tokens and a
@@ -46,7 +47,7 @@ __global__ void __launch_bounds__(kRowWaves* kWave, 1) kv_rows_kernel(KvParams p
     for (uint32_t i = i_begin + wave; i < i_end; i += kRowWaves) {
         const uint32_t tok0 = seen.tile(i) * T::kTokens;
         T tile;
-        const auto rows = T::rows_of(p, table, kvh, tok0, seen, lane);
+        const auto rows = T::rows_from(p, T::entry_of(p, table, tok0, seen, lane), kvh, tok0, seen, lane);
         tile.load(p, rows, kvh, lane);
         const bool masked = T::needs_mask(p, rows, tok0, lo_all, hi_all);
         attend_tile<kQF32, kF8, kRows, kD, true>(p, tile, rows, tok0, seen, lo, hi, masked, st, lane);
@@ -269,6 +270,14 @@ int launch_decode_ex(const granite_hip_decode_args& a, const granite_hip_kv_form
     p.decode = 1;
     p.causal = 1;
     p.scale_log2 = a.scale * kExLog2e;
+    p.q_groups = (p.group + 15) / 16;
+    // Tiles of the longest sequence: its whole length, or its window and sinks and the tiles their ends lie in.
+    const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3;
+    const uint32_t tile = f8 ? 64 : 32;
+    const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + 2 * tile) : p.max_tokens;
+    const uint32_t tiles = uint32_t((seen + tile - 1) / tile);
+    if (tiles > kDirectTiles && kv_stream_supports(p, tiles))
+        return launch_kv_stream(p, D, a.q_dtype == GRANITE_HIP_F32, f8, rows, tiles, scratch);
     return launch_rows(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
 }
 

@@ -50,6 +50,9 @@ struct KvParams {
     float q_sign;  // tiles kernel: 1, -1 or 0, taken into Q
 };
 
+// decode_ex_stream.hip: the persistent decode kernel.  tiles_per_seq: most tiles a sequence can have to visit.
+bool kv_stream_supports(const KvParams& p, uint32_t tiles_per_seq);
+int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t tiles_per_seq, const ScratchSource& scratch);
 // attention_ex.hip: the tiles kernel.  Block sizes are multiples of 16, or the cache is contiguous.
 int launch_kv_tiles(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const ScratchSource& scratch);
 
@@ -119,42 +122,57 @@ struct Tile {
     // tok0: first token of the tile.  `seen`: what the launch's or workgroup's queries see between
     // them; the block table is not looked up beyond its end, and rows none of them sees have scale 0
     // (whatever lies in the scale array there must not count as the largest).
-    // Whether some row that sees [lo, hi) and the sinks does not see some token of the tile, invalid pages
-    // included (uniform).
+    // In two steps, so that the table entry can be in flight while other loads are issued.
+    // needs_mask: whether some row that sees [lo, hi) and the sinks does not see some token of the tile,
+    // invalid pages included (uniform).
     static __device__ __forceinline__ bool needs_mask(const KvParams& p, const Rows& r, uint32_t tok0, uint32_t lo, uint32_t hi) {
         bool m = tok0 + kTokens > hi || (tok0 < lo && tok0 + kTokens > p.sinks);
         if constexpr (kRows != kExContiguous) m = m || __any(r.valid == 0);
         return m;
     }
-
-    static __device__ __forceinline__ Rows rows_of(const KvParams& p, const int32_t* table, uint32_t kvh,
-                                                   uint32_t tok0, const VisibleTiles& seen, uint32_t lane) {
+    struct Entry {
+        int32_t entry;
+        uint32_t in;  // row in the block; contiguous: the row
+    };
+    static __device__ __forceinline__ uint32_t first_of(uint32_t tok0, uint32_t lane) {
+        return kRows == kExPaged16 ? tok0 + 16 * (lane & (kSubs - 1)) : tok0 + (lane & (kTokens - 1));
+    }
+    static __device__ __forceinline__ Entry entry_of(const KvParams& p, const int32_t* table, uint32_t tok0,
+                                                     const VisibleTiles& seen, uint32_t lane) {
+        Entry e;
+        const uint32_t tok = min(first_of(tok0, lane), seen.end - 1);
+        if constexpr (kRows == kExContiguous) {
+            e.entry = 0;
+            e.in = tok;
+        } else {
+            uint32_t blk;
+            if (p.bs_shift >= 0) {
+                blk = tok >> p.bs_shift;
+                e.in = tok & (p.block_size - 1);
+            } else {
+                blk = tok / p.block_size;
+                e.in = tok - blk * p.block_size;
+            }
+            // (a run whose first token is clamped is addressed from its start all the same)
+            if constexpr (kRows == kExPaged16) e.in &= ~15u;
+            e.entry = table[blk];
+        }
+        return e;
+    }
+    static __device__ __forceinline__ Rows rows_from(const KvParams& p, const Entry& e, uint32_t kvh, uint32_t tok0,
+                                                     const VisibleTiles& seen, uint32_t lane) {
         Rows r;
         r.ks = r.vs = 1.0f;
         r.valid = 1;
-        const uint32_t last = seen.end - 1;
         if constexpr (kRows == kExContiguous) {
-            r.row = min(tok0 + (lane & (kTokens - 1)), last);
+            r.row = e.in;
         } else {
-            const uint32_t first = kRows == kExPaged16 ? tok0 + 16 * (lane & (kSubs - 1)) : tok0 + (lane & (kTokens - 1));
-            const uint32_t tok = min(first, last);
-            uint32_t blk, in;
-            if (p.bs_shift >= 0) {
-                blk = tok >> p.bs_shift;
-                in = tok & (p.block_size - 1);
-            } else {
-                blk = tok / p.block_size;
-                in = tok - blk * p.block_size;
-            }
-            // (a run whose first token is clamped to `last` keeps the clamped token's place in its
-            // 16-token run out of the row: the run is addressed from its start)
-            if constexpr (kRows == kExPaged16) in &= ~15u;
-            const int32_t entry = table[blk];
-            r.valid = pool_row(entry, in, p.block_size, p.num_blocks, &r.row) ? 1u : 0u;
+            r.valid = pool_row(e.entry, e.in, p.block_size, p.num_blocks, &r.row) ? 1u : 0u;
             if constexpr (kF8) {
-                const size_t at = size_t(r.valid ? uint32_t(entry) : 0u) * p.num_kv_heads + kvh;
-                const bool used = r.valid && first <= last &&
-                                  (first + (kRows == kExPaged16 ? 15 : 0) >= seen.lo || first < p.sinks);
+                const uint32_t first = first_of(tok0, lane);
+                const size_t at = size_t(r.valid ? uint32_t(e.entry) : 0u) * p.num_kv_heads + kvh;
+                const bool used = bool(int(r.valid) & int(first < seen.end) &
+                                       (int(first + (kRows == kExPaged16 ? 15 : 0) >= seen.lo) | int(first < p.sinks)));
                 const float ks = p.k_scale[at], vs = p.v_scale[at];
                 r.ks = used ? ks : 0.0f;
                 r.vs = used ? vs : 0.0f;
