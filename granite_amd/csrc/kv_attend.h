@@ -94,8 +94,8 @@ __device__ __forceinline__ uint32_t ex_seq_len(const KvParams& p, uint32_t b) {
 //
 // A tile is 64 tokens of an 8-bit cache or 32 of a half one: 64 registers of K and V per lane either
 // way.  K is the A operand as it lies in memory; the head-dim elements a lane holds for step s are
-// d_of(s, g) .. + 7, an order that only Q has to share: with 8 bits a lane reads a quarter of a row
-// in 16-byte pieces.  V^T takes the tokens of a step in the order 4 g + j, 16 + 4 g + j, which is how the first
+// d_of(s, g) .. + 7, an order that only Q has to share: the four lanes of a row read 64 consecutive bytes per
+// instruction in either type.  V^T takes the tokens of a step in the order 4 g + j, 16 + 4 g + j, which is how the first
 // product leaves the probabilities, and is put together from 4 x 4 byte (8 x 2 half) transposes with
 // v_perm_b32; row m of output tile t is d = 8 m + t, so a lane ends with 32 consecutive elements.
 // At head size 64 lanes 8 .. 15 of a group repeat the V loads of lanes 0 .. 7 and what they compute is dropped.
@@ -109,7 +109,7 @@ struct Tile {
     static constexpr int kVWords = kF8 ? 2 : 4;
 
     static __device__ __forceinline__ uint32_t d_of(int s, uint32_t g) {
-        return kF8 ? (kD / 4) * g + 8 * s : 32 * s + 8 * g;
+        return kF8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
     }
 
     // Rows of a tile.  Paged16: lane l holds the row of token 16 (l & 3) of the tile (its 16-token
@@ -184,47 +184,69 @@ struct Tile {
     uint4v ka[kSubs][kKLoads];
     uint32_t vr[kSubs * 4][kVWords];  // token 16 (j / 4) + 4 g + j % 4 at d = 8 n
 
+    // Paged16: a run of 16 rows is a buffer of its own whose base is scalar (pools may exceed the 4 GiB an offset
+    // reaches, a run cannot), so a load needs no vector arithmetic: the lane's offset inside the run, the same for every
+    // run, plus a scalar for the row of four (V) or an immediate (K).
     __device__ __forceinline__ void load(const KvParams& p, const Rows& r, uint32_t kvh, uint32_t lane) {
         const uint32_t n = lane & 15, g = lane >> 4;
         const uint8_t* kb = p.k + int64_t(kvh) * p.head_bytes;
         const uint8_t* vb = p.v + int64_t(kvh) * p.head_bytes;
         constexpr uint32_t kElem = kF8 ? 1 : 2;
         const uint32_t k_in = kElem * d_of(0, g), v_in = kElem * 8 * (n & (kD / 8 - 1));
+        if constexpr (kRows == kExPaged16) {
+            const uint32_t row_bytes = uint32_t(p.row_bytes);
+            const int k_off = int(n * row_bytes + k_in), v_off = int(4 * g * row_bytes + v_in);
 #pragma unroll
-        for (int sub = 0; sub < kSubs; sub++) {
-            const uint8_t* kp;
-            if constexpr (kRows == kExPaged16) {
-                const uint32_t row = uint32_t(__builtin_amdgcn_readlane(int(r.row), sub));
-                kp = kb + uint64_t(row) * uint64_t(p.row_bytes) + (uint32_t(n) * uint32_t(p.row_bytes) + k_in);
-            } else {
-                kp = kb + uint64_t(ex_lane_read(r.row, 16 * sub + n)) * uint64_t(p.row_bytes) + k_in;
+            for (int sub = 0; sub < kSubs; sub++) {
+                const uint64_t at = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(r.row), sub))) * row_bytes;
+                const auto run = run_of(kb + at, row_bytes);
+#pragma unroll
+                for (int i = 0; i < kKLoads; i++)
+                    ka[sub][i] = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(run, k_off, 64 * i, 0));
             }
 #pragma unroll
-            for (int i = 0; i < kKLoads; i++)
-                ka[sub][i] = *reinterpret_cast<const uint4v*>(kp + (kF8 ? 16 : 64) * i);
+            for (int sub = 0; sub < kSubs; sub++) {
+                const uint64_t at = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(r.row), sub))) * row_bytes;
+                const auto run = run_of(vb + at, row_bytes);
+                // every byte of V is used once: streaming loads (bit 1 of the last operand)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (kF8) {
+                        const uint2v w = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(run, v_off, int(j * row_bytes), 2));
+                        vr[4 * sub + j][0] = w.x;
+                        vr[4 * sub + j][1] = w.y;
+                    } else {
+                        const uint4v w = __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(run, v_off, int(j * row_bytes), 2));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) vr[4 * sub + j][i] = w[i];
+                    }
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++) {
+            const uint8_t* kp = kb + uint64_t(ex_lane_read(r.row, 16 * sub + n)) * uint64_t(p.row_bytes) + k_in;
+#pragma unroll
+            for (int i = 0; i < kKLoads; i++) ka[sub][i] = *reinterpret_cast<const uint4v*>(kp + 64 * i);
         }
 #pragma unroll
         for (int j = 0; j < kSubs * 4; j++) {
-            const uint8_t* vp;
-            if constexpr (kRows == kExPaged16) {
-                const uint32_t row = uint32_t(__builtin_amdgcn_readlane(int(r.row), j / 4));
-                vp = vb + uint64_t(row) * uint64_t(p.row_bytes) + ((4 * g + j % 4) * uint32_t(p.row_bytes) + v_in);
-            } else {
-                vp = vb + uint64_t(ex_lane_read(r.row, 16 * (j / 4) + 4 * g + j % 4)) * uint64_t(p.row_bytes) + v_in;
-            }
-            // every byte of V is used once: streaming loads
+            const uint8_t* vp = vb + uint64_t(ex_lane_read(r.row, 16 * (j / 4) + 4 * g + j % 4)) * uint64_t(p.row_bytes) + v_in;
             if constexpr (kF8) {
                 const uint2v w = __builtin_nontemporal_load(reinterpret_cast<const uint2v*>(vp));
                 vr[j][0] = w.x;
                 vr[j][1] = w.y;
             } else {
                 const uint4v w = __builtin_nontemporal_load(reinterpret_cast<const uint4v*>(vp));
-                vr[j][0] = w.x;
-                vr[j][1] = w.y;
-                vr[j][2] = w.z;
-                vr[j][3] = w.w;
+#pragma unroll
+                for (int i = 0; i < 4; i++) vr[j][i] = w[i];
             }
         }
+    }
+    // The 16 rows from `first` on as a buffer: raw 32-bit elements, reads behind its end give zero.
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t run_of(const uint8_t* first, uint32_t row_bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(first), 0, int(16 * row_bytes), 0x00020000);
     }
 
     // A operand of the first product: step s of sub-tile `sub`
@@ -322,6 +344,15 @@ struct Rows16 {
     }
 };
 
+// The maximum over the four lanes n, n + 16, n + 32, n + 48, in all of them: two register swaps, no LDS round trip
+// (v_permlane16_swap exchanges the odd rows of 16 lanes of one register with the even rows of the other).
+__device__ __forceinline__ float max_over_groups(float v) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    const LanePair both = half_wave_pair(fmaxf(a, b));
+    return fmaxf(both.lo, both.hi);
+}
+
 // One tile's contribution to the rows of `st`.  `seen` is what all rows see between them, [lo, hi) and
 // the first `sinks` tokens what the lane's own row sees.  `masked` (uniform): some row does not see some
 // token of the tile.  kPerRow: the rows differ in what they see.
@@ -358,7 +389,7 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
     }
     uint32_t visible = 0xFFFFu;  // bit 4 sub + i: the lane's row sees token 16 sub + 4 g + i
     if (masked) {
-        visible = 0;
+        if constexpr (kPerRow) visible = 0;
 #pragma unroll
         for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
@@ -368,20 +399,23 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
                                        : kRows == kExPaged16  ? uint32_t(__builtin_amdgcn_readlane(int(rows.valid), sub))
                                                               : ex_lane_read(rows.valid, in);
                 const bool vis = bool(int(valid) & int(tok < hi) & (int(tok >= lo) | int(tok < p.sinks)));
-                if (vis) visible |= 1u << (4 * sub + i);
-                else s[sub][i] = -INFINITY;
+                if constexpr (kPerRow) visible |= vis ? 1u << (4 * sub + i) : 0u;
+                s[sub][i] = vis ? s[sub][i] : -INFINITY;
                 const bool any = kPerRow ? bool(int(valid) & int(tok < seen.end) & (int(tok >= seen.lo) | int(tok < p.sinks))) : vis;
-                if (!any) {
+                // (pinned here: moved behind the branch, the selects and the conditions they need would be paid for by
+                // every tile)
+                asm volatile("" : "+v"(s[sub][i]));
 #pragma unroll
-                    for (int w = 0; w < T::kVWords; w++) tile.vr[4 * sub + i][w] = 0;
+                for (int w = 0; w < T::kVWords; w++) {
+                    tile.vr[4 * sub + i][w] = any ? tile.vr[4 * sub + i][w] : 0u;
+                    asm volatile("" : "+v"(tile.vr[4 * sub + i][w]));
                 }
             }
     }
     float top = s[0][0];
 #pragma unroll
     for (int i = 1; i < 4 * kSubs; i++) top = fmaxf(top, s[i / 4][i % 4]);
-    top = fmaxf(top, wave_shfl_xor(top, 16));
-    top = fmaxf(top, wave_shfl_xor(top, 32));
+    top = max_over_groups(top);
     const float m_new = fmaxf(st.m, top);
     float rescale = fast_exp2(st.m - m_new);  // of O; of l without the change of the V scale
     st.l *= rescale;
