@@ -18,7 +18,7 @@ HOST = PKG / "host"
 LIBDIR = PKG / "lib"
 BINDIR = PKG / "bin"
 
-HIP_SOURCES = ["capi.hip", "kv_ops.hip", "rope.hip", "rope_q8.hip", "qkv_q4k.hip", "decode.hip", "decode_stream.hip", "decode_ex.hip", "decode_ex_stream.hip", "attention_ex.hip", "prefill.hip", "prefill_dma.hip"]
+HIP_SOURCES = ["capi.hip", "kv_ops.hip", "rope.hip", "rope_q8.hip", "qkv_q4k.hip", "decode.hip", "decode_stream.hip", "decode_ex.hip", "decode_ex_stream.hip", "decode_ex_dma.hip", "attention_ex.hip", "prefill.hip", "prefill_dma.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

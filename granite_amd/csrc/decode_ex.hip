@@ -9,7 +9,7 @@ namespace ghip {
 namespace {
 
 constexpr uint32_t kRowWaves = 4;
-constexpr uint32_t kDirectTiles = 12;
+constexpr uint32_t kDirectTokens = 768;
 
 // One workgroup per (run of 16 query rows, KV head, sequence, key split).  A row is a (query, head of
 // the KV head's group) pair, row r = query * group + head, so a decode step's group, a few draft tokens and a
@@ -273,10 +273,10 @@ int launch_decode_ex(const granite_hip_decode_args& a, const granite_hip_kv_form
     p.q_groups = (p.group + 15) / 16;
     // Tiles of the longest sequence: its whole length, or its window and sinks and the tiles their ends lie in.
     const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3;
-    const uint32_t tile = f8 ? 64 : 32;
+    const uint32_t tile = kv_stream_tile(p, f8, rows);
     const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + 2 * tile) : p.max_tokens;
     const uint32_t tiles = uint32_t((seen + tile - 1) / tile);
-    if (tiles > kDirectTiles && kv_stream_supports(p, tiles))
+    if (tiles * tile > kDirectTokens && kv_stream_supports(p, tiles))
         return launch_kv_stream(p, D, a.q_dtype == GRANITE_HIP_F32, f8, rows, tiles, scratch);
     return launch_rows(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
 }

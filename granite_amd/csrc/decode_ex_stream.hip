@@ -291,6 +291,11 @@ void launch_cache(const KvParams& p, uint32_t per_list, dim3 grid, size_t lds, b
 
 }  // namespace
 
+uint32_t kv_stream_tile(const KvParams& p, bool f8, int rows) {
+    if (!f8) return 32;
+    return rows == kExPaged16 && p.batch <= kDmaMaxBatch ? 32 : 64;
+}
+
 bool kv_stream_supports(const KvParams& p, uint32_t tiles_per_seq) {
     const uint64_t units = uint64_t(p.batch) * tiles_per_seq * p.num_kv_heads * p.q_groups;
     return p.batch + 1 <= kMaxPrefix && units < (1ull << 31) && p.num_heads <= 0x7FFFFFFFu && p.batch <= 65535u;
@@ -321,7 +326,9 @@ int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint
     {
         KernelTimerScope timer("decode_ex");
         const dim3 grid(cus);
-        if (D == 128) {
+        if (kv_stream_tile(p, f8, rows) == 32 && f8) {
+            if (int rc = launch_kv_dma(p, D, q_f32, per_list, grid)) return rc;
+        } else if (D == 128) {
             if (q_f32) launch_cache<true, 128>(p, per_list, grid, lds, f8, rows);
             else launch_cache<false, 128>(p, per_list, grid, lds, f8, rows);
         } else {
