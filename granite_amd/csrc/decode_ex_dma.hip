@@ -185,9 +185,6 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
     cur = plan_tiles(0);
     wait_transfers<0>();
     plan_rows(cur);
-    wait_transfers<0>();
-    plan_scales(cur);
-    next = cur;
 
     // ---- a tile on its way: what is read from the plan when it is requested
     struct Unit {
@@ -210,10 +207,6 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
         u.b = lane_u(cur.b, l);
         u.lh = lane_u(cur.lh, l);
         u.valid = lane_u(cur.valid, l) | (lane_u(cur.valid, l + 1) << 1);
-        u.ks[0] = lane_f(cur.ks, l);
-        u.ks[1] = lane_f(cur.ks, l + 1);
-        u.vs[0] = lane_f(cur.vs, l);
-        u.vs[1] = lane_f(cur.vs, l + 1);
         const uint64_t head = uint64_t(kv_head_of(u.lh)) * uint64_t(p.head_bytes);
         const uint32_t dst = lds_wave + buf * 2 * G::kHalf;
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the buffer's last reads are through
@@ -230,6 +223,14 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
             }
         }
         return u;
+    };
+
+    auto take_scales = [&](uint32_t i, Unit& u) __attribute__((always_inline)) {
+        const uint32_t l = 2 * (i % kPlanUnits);
+        u.ks[0] = lane_f(cur.ks, l);
+        u.ks[1] = lane_f(cur.ks, l + 1);
+        u.vs[0] = lane_f(cur.vs, l);
+        u.vs[1] = lane_f(cur.vs, l + 1);
     };
 
     // ---- query rows and running state, as Rows16
@@ -401,9 +402,16 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
     };
 
     clear();
+    // (the first tiles do not wait for their scales, which were requested before them)
     Unit now = request(0, 0), then = now;
-    load_q(now);
     if (n_units > 1) then = request(1, 1);
+    load_q(now);
+    if (n_units > 1) wait_transfers<2 * G::kTransfers>();
+    else wait_transfers<G::kTransfers>();
+    plan_scales(cur);
+    next = cur;
+    take_scales(0, now);
+    take_scales(min(1u, n_units - 1), then);
     for (uint32_t i = 0; i < n_units; i++) {
         if (i + 1 < n_units) wait_transfers<G::kTransfers>();  // all but the next tile's
         else wait_transfers<0>();
@@ -418,6 +426,7 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
         if (j < n_units) {
             if (j % kPlanUnits == 0) cur = next;
             then = request(j, i & 1);
+            take_scales(j, then);
             // the next 32 tiles' plan, in three steps a few tiles apart: what a step needs was requested by the one before
             // and is older than the last tile's transfers, which the loop waits for
             const uint32_t at = j % kPlanUnits;

@@ -207,10 +207,10 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_stream_kernel(KvParams p)
 }
 
 // Joins the pieces of one (sequence, query head): the workers that touched its list head are consecutive.  kJoin
-// groups of threads take four pieces at a time in turn (a long sequence alone has a piece of every worker) and are
-// joined through LDS.
-constexpr uint32_t kJoin = 4;
-template <int kD>
+// groups of threads take four pieces at a time in turn and are joined through LDS: 4 where sequences are few (a long
+// one alone has a piece of every worker: 2 sequences of 131072 tokens 17.5 -> 7.3 us), 1 where they are many and short
+// of pieces (64 sequences: 5.3 us against 6.8).
+template <int kD, uint32_t kJoin>
 __global__ void __launch_bounds__(kD* kJoin) kv_stream_merge_kernel(KvParams p) {
     const uint32_t qh = blockIdx.x, b = blockIdx.y, d = threadIdx.x % kD, part = threadIdx.x / kD;
     const uint32_t* prefix = p.plan + kPlanHeader;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kD* kJoin) kv_stream_merge_kernel(KvParams p) 
         }
         mx = m_new;
     }
-    if (n_parts > 4) {  // uniform
+    if (kJoin > 1 && n_parts > 4) {  // uniform
         __shared__ float s_o[kJoin][kD], s_m[kJoin], s_l[kJoin];
         s_o[part][d] = o;
         if (d == 0) {
@@ -340,8 +340,12 @@ int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint
     {
         KernelTimerScope timer("decode_ex_merge");
         const dim3 grid(p.num_heads, p.batch);
-        if (D == 128) kv_stream_merge_kernel<128><<<grid, dim3(128 * kJoin), 0, ctx().stream>>>(p);
-        else kv_stream_merge_kernel<64><<<grid, dim3(64 * kJoin), 0, ctx().stream>>>(p);
+        const bool few = size_t(p.batch) * lists * 16 <= p.workers;  // 16 pieces a segment or more if all are as long
+        hipStream_t st = ctx().stream;
+        if (D == 128 && few) kv_stream_merge_kernel<128, 4><<<grid, dim3(512), 0, st>>>(p);
+        else if (D == 128) kv_stream_merge_kernel<128, 1><<<grid, dim3(128), 0, st>>>(p);
+        else if (few) kv_stream_merge_kernel<64, 4><<<grid, dim3(256), 0, st>>>(p);
+        else kv_stream_merge_kernel<64, 1><<<grid, dim3(64), 0, st>>>(p);
     }
     return launch_status();
 }
