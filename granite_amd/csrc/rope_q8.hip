@@ -15,9 +15,9 @@
 // One launch of up to three kinds of workgroups:
 //   * run of tokens of one sequence: a workgroup per (block the run touches, KV head).  Its four waves
 //     take the block's new rows in turn and keep them in registers between the maximum and the
-//     codes (blocks of up to 64 rows of 128 or 128 rows of 64 elements; what is beyond is read twice),
+//     codes (blocks of up to 32 rows of 128 or 64 rows of 64 elements; what is beyond is read twice),
 //   * one token per sequence: a wave per (token, KV head), K in its lower half and V in its upper,
-//   * Q: a thread per four elements of a token's row in one or kQHeads heads, cos and sin loaded once for all.
+//   * Q: a thread per eight elements of a token's row in one or kQHeads heads, cos and sin loaded once for all.
 #include <cmath>
 
 #include "common.h"
@@ -27,7 +27,7 @@ namespace ghip {
 namespace {
 
 constexpr uint32_t kThreads = 256, kWaves = 4;
-constexpr int kHold = 8;         // passes of a wave over new rows that stay in registers
+constexpr int kHold = 4;         // passes of a wave over new rows that stay in registers
 constexpr uint32_t kQHeads = 4;  // heads per thread of the Q part of a large launch
 constexpr float kF8Max = 448.0f;
 
@@ -71,6 +71,21 @@ __device__ __forceinline__ Quad load_quad(const void* base, size_t at) {  // rea
         for (int i = 0; i < 4; i++) r.x[i] = f[i];
     }
     return r;
+}
+
+template <bool kF16>
+__device__ __forceinline__ void load_oct(const void* base, size_t at, Quad& lo, Quad& hi) {
+    if constexpr (kF16) {
+        const half8 h = __builtin_nontemporal_load(reinterpret_cast<const half8*>(static_cast<const _Float16*>(base) + at));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            lo.x[i] = static_cast<float>(h[i]);
+            hi.x[i] = static_cast<float>(h[4 + i]);
+        }
+    } else {
+        lo = load_quad<false>(base, at);
+        hi = load_quad<false>(base, at + 4);
+    }
 }
 
 struct Angles {
@@ -281,30 +296,40 @@ __device__ void append_step(const RopeQ8Params& p) {
     }
 }
 
+// A thread has eight consecutive elements of a row, 16 bytes of halves, in q_heads heads; the loads of all of them and
+// of their angles are in flight together.
 template <bool kSrcF16, int kD>
 __device__ void rotate_q(const RopeQ8Params& p) {
-    constexpr uint32_t kQuads = kD / 4;
+    constexpr uint32_t kOcts = kD / 8;
     const uint32_t runs = (p.num_heads_q + p.q_heads - 1) / p.q_heads;
     const uint64_t idx = uint64_t(blockIdx.x - p.kv_groups) * kThreads + threadIdx.x;
-    const uint32_t j = uint32_t(idx % kQuads);
-    const uint64_t rest = idx / kQuads;
-    const uint32_t run = uint32_t(rest % runs), s = uint32_t(rest / runs);
-    if (rest / runs >= p.seq_len) return;
+    const uint32_t j = uint32_t(idx % kOcts);
+    const uint64_t rest = idx / kOcts;
+    if (rest >= uint64_t(runs) * p.seq_len) return;
+    const uint32_t s = uint32_t(rest / runs), run = uint32_t(rest - uint64_t(s) * runs);
     uint32_t pos;
     if (!position_of(p, s, &pos)) return;
-    const Angles ang = angles_of(p, pos, j, kD);
-    const uint32_t h0 = run * p.q_heads, h1 = min(h0 + p.q_heads, p.num_heads_q);
-    Quad x[kQHeads];
-#pragma unroll
-    for (uint32_t i = 0; i < kQHeads; i++)
-        if (h0 + i < h1) x[i] = load_quad<kSrcF16>(p.q, (size_t(s) * p.num_heads_q + h0 + i) * kD + 4 * j);
+    const uint32_t h0 = run * p.q_heads;
+    const size_t at0 = (size_t(s) * p.num_heads_q + h0) * kD + 8 * j;
+    Quad lo[kQHeads], hi[kQHeads];
 #pragma unroll
     for (uint32_t i = 0; i < kQHeads; i++) {
-        if (h0 + i >= h1) continue;
-        const Quad r = rotate(x[i], ang);
-        const size_t at = (size_t(s) * p.num_heads_q + h0 + i) * kD + 4 * j;
-        if (p.q_out_f32) *reinterpret_cast<float4v*>(static_cast<float*>(p.q_out) + at) = float4v{r.x[0], r.x[1], r.x[2], r.x[3]};
-        else *reinterpret_cast<uint2v*>(static_cast<uint16_t*>(p.q_out) + at) = uint2v{pack_f16x2(r.x[0], r.x[1]), pack_f16x2(r.x[2], r.x[3])};
+        if (i < p.q_heads && h0 + i < p.num_heads_q) load_oct<kSrcF16>(p.q, at0 + i * kD, lo[i], hi[i]);
+    }
+    const Angles a0 = angles_of(p, pos, 2 * j, kD), a1 = angles_of(p, pos, 2 * j + 1, kD);
+#pragma unroll
+    for (uint32_t i = 0; i < kQHeads; i++) {
+        if (i >= p.q_heads || h0 + i >= p.num_heads_q) continue;
+        const Quad r0 = rotate(lo[i], a0), r1 = rotate(hi[i], a1);
+        const size_t at = at0 + i * kD;
+        if (p.q_out_f32) {
+            float4v* out = reinterpret_cast<float4v*>(static_cast<float*>(p.q_out) + at);
+            out[0] = float4v{r0.x[0], r0.x[1], r0.x[2], r0.x[3]};
+            out[1] = float4v{r1.x[0], r1.x[1], r1.x[2], r1.x[3]};
+        } else {
+            *reinterpret_cast<uint4v*>(static_cast<uint16_t*>(p.q_out) + at) =
+                uint4v{pack_f16x2(r0.x[0], r0.x[1]), pack_f16x2(r0.x[2], r0.x[3]), pack_f16x2(r1.x[0], r1.x[1]), pack_f16x2(r1.x[2], r1.x[3])};
+        }
     }
 }
 
@@ -383,11 +408,11 @@ int launch_rope_append_q8(const granite_hip_rope_q8_args& a) {
         kv_groups = a.positions ? (units * a.num_heads_k + kWaves - 1) / kWaves : units * a.num_heads_k;
     }
     if (a.q) {
-        const uint64_t quads = uint64_t(a.seq_len) * (a.head_dim / 4) * a.num_heads_q;
+        const uint64_t octs = uint64_t(a.seq_len) * (a.head_dim / 8) * a.num_heads_q;
         // one head per thread until there are four times as many threads as the part holds at once
         // (256 CUs x 2048): the lookup of cos and sin is then shared by four heads
-        p.q_heads = quads >= (2ull << 20) ? kQHeads : 1;
-        const uint64_t threads = uint64_t(a.seq_len) * (a.head_dim / 4) * ((a.num_heads_q + p.q_heads - 1) / p.q_heads);
+        p.q_heads = octs >= (2ull << 20) ? kQHeads : 1;
+        const uint64_t threads = uint64_t(a.seq_len) * (a.head_dim / 8) * ((a.num_heads_q + p.q_heads - 1) / p.q_heads);
         q_groups = (threads + kThreads - 1) / kThreads;
     }
     if (kv_groups + q_groups > 0x7FFFFFFFull) return GRANITE_HIP_EINVAL;
