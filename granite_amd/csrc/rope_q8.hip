@@ -13,9 +13,9 @@
 // against top / 448, x / scale is exact, and growing a scale is exact as well for codes that stay above 2^-6.
 //
 // One launch of up to three kinds of workgroups:
-//   * run of tokens of one sequence: a workgroup per (block the run touches, KV head).  Its four waves
-//     take the block's new rows in turn and keep them in registers between the maximum and the
-//     codes (blocks of up to 32 rows of 128 or 64 rows of 64 elements; what is beyond is read twice),
+//   * run of tokens of one sequence: one, two or four waves per (block the run touches, KV head), by the block
+//     size.  They take the block's new rows in turn and keep them in registers between the maximum and the
+//     codes (8 rows of 128 or 16 of 64 elements a wave; what four waves cannot hold is read twice),
 //   * one token per sequence: a wave per (token, KV head), K in its lower half and V in its upper,
 //   * Q: a thread per eight elements of a token's row in one or kQHeads heads, cos and sin loaded once for all.
 #include <cmath>
@@ -27,8 +27,8 @@ namespace ghip {
 namespace {
 
 constexpr uint32_t kThreads = 256, kWaves = 4;
-constexpr int kHold = 4;         // passes of a wave over new rows that stay in registers
-constexpr uint32_t kQHeads = 4;  // heads per thread of the Q part of a large launch
+constexpr int kHold = 2;         // passes of a wave over new rows that stay in registers
+constexpr uint32_t kQHeads = 2;  // heads per thread of the Q part of a large launch
 constexpr float kF8Max = 448.0f;
 
 struct RopeQ8Params {
@@ -51,11 +51,15 @@ struct RopeQ8Params {
     uint32_t block_size, num_blocks, max_blocks;
     uint32_t kv_groups;  // workgroups of the K/V part, in front of those of the Q part
     uint32_t q_heads;    // heads per thread of the Q part
+    uint32_t kv_units, unit_waves;  // run form: (block, head) pairs, and how many of a workgroup's waves share one
     int q_out_f32;
 };
 
 struct Quad {
     float x[4];
+};
+struct Oct {
+    Quad lo, hi;
 };
 
 template <bool kF16>
@@ -156,88 +160,97 @@ __device__ __forceinline__ float wave_max(float v, int from) {
 
 template <bool kSrcF16, int kD>
 __device__ void append_run(const RopeQ8Params& p) {
-    constexpr uint32_t kQuads = kD / 4, kRowsPerPass = 64 / kQuads;
-    __shared__ float s_top[2][kWaves];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t head = blockIdx.x % p.num_heads_k, nth = blockIdx.x / p.num_heads_k;
-    const uint32_t first_block = p.start_pos / p.block_size, blk = first_block + nth;
+    constexpr uint32_t kOcts = kD / 8, kRowsPerPass = 64 / kOcts;
+    __shared__ float s_top[kWaves][2];
+    const uint32_t lane = threadIdx.x & 63, wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
+    const uint32_t part = wave % p.unit_waves;  // of the waves that share a unit
+    const uint32_t unit = min(blockIdx.x * (kWaves / p.unit_waves) + wave / p.unit_waves, p.kv_units - 1);
+    const bool spare = blockIdx.x * (kWaves / p.unit_waves) + wave / p.unit_waves >= p.kv_units;
+    const uint32_t head = unit % p.num_heads_k, blk = p.start_pos / p.block_size + unit / p.num_heads_k;
     const uint32_t end = p.start_pos + p.seq_len;
     const uint32_t lo = max(p.start_pos, blk * p.block_size), hi = min(end, (blk + 1) * p.block_size);  // positions
-    uint32_t row0;  // pool row of position lo; the block's first row is row0 - (lo - blk * block_size)
     const int32_t entry = p.table[blk];
-    if (!pool_row(entry, lo - blk * p.block_size, p.block_size, p.num_blocks, &row0)) return;  // uniform
-    const uint32_t j = lane % kQuads, sub = lane / kQuads;
+    const uint32_t j = lane % kOcts, sub = lane / kOcts;
     const uint32_t n_rows = hi - lo;
 
-    auto fetch = [&](uint32_t i, Quad& k, Quad& v) {  // new row i of the block
+    auto fetch = [&](uint32_t i, Oct& k, Oct& v) {  // new row i of the block
         const uint32_t s = lo + i - p.start_pos;
-        const size_t at = (size_t(s) * p.num_heads_k + head) * kD + 4 * j;
-        k = rotate(load_quad<kSrcF16>(p.k, at), angles_of(p, lo + i, j, kD));
-        v = load_quad<kSrcF16>(p.v, at);
+        const size_t at = (size_t(s) * p.num_heads_k + head) * kD + 8 * j;
+        load_oct<kSrcF16>(p.k, at, k.lo, k.hi);
+        load_oct<kSrcF16>(p.v, at, v.lo, v.hi);
     };
-    Quad kq[kHold], vq[kHold];
+    auto turn = [&](uint32_t i, Oct& k) {
+        k.lo = rotate(k.lo, angles_of(p, lo + i, 2 * j, kD));
+        k.hi = rotate(k.hi, angles_of(p, lo + i, 2 * j + 1, kD));
+    };
+    Oct kq[kHold], vq[kHold];
     float k_top = 0.0f, v_top = 0.0f;
-    const uint32_t stride = kWaves * kRowsPerPass;
+    const uint32_t stride = p.unit_waves * kRowsPerPass, first = part * kRowsPerPass + sub;
+#pragma unroll
+    for (int h = 0; h < kHold; h++)
+        if (h * stride + first < n_rows) fetch(h * stride + first, kq[h], vq[h]);
+    const size_t scale_at = size_t(uint32_t(entry) < p.num_blocks ? uint32_t(entry) : 0u) * p.num_heads_k + head;
+    const uint32_t kept = lo - blk * p.block_size;  // rows in front of the new ones
+    const float k_old = kept ? p.k_scale[scale_at] : 0.0f, v_old = kept ? p.v_scale[scale_at] : 0.0f;
 #pragma unroll
     for (int h = 0; h < kHold; h++) {
-        const uint32_t i = h * stride + wave * kRowsPerPass + sub;
-        if (i < n_rows) {
-            fetch(i, kq[h], vq[h]);
-            k_top = finite_top(kq[h], k_top);
-            v_top = finite_top(vq[h], v_top);
+        if (h * stride + first < n_rows) {
+            turn(h * stride + first, kq[h]);
+            k_top = finite_top(kq[h].hi, finite_top(kq[h].lo, k_top));
+            v_top = finite_top(vq[h].hi, finite_top(vq[h].lo, v_top));
         }
     }
-    for (uint32_t i = kHold * stride + wave * kRowsPerPass + sub; i < n_rows; i += stride) {
-        Quad k, v;
+    for (uint32_t i = kHold * stride + first; i < n_rows; i += stride) {
+        Oct k, v;
         fetch(i, k, v);
-        k_top = finite_top(k, k_top);
-        v_top = finite_top(v, v_top);
+        turn(i, k);
+        k_top = finite_top(k.hi, finite_top(k.lo, k_top));
+        v_top = finite_top(v.hi, finite_top(v.lo, v_top));
     }
     k_top = wave_max(k_top, 32);
     v_top = wave_max(v_top, 32);
-    if (lane == 0) {
-        s_top[0][wave] = k_top;
-        s_top[1][wave] = v_top;
+    if (p.unit_waves > 1) {  // uniform over the launch
+        if (lane == 0) {
+            s_top[wave][0] = k_top;
+            s_top[wave][1] = v_top;
+        }
+        __syncthreads();
+        for (uint32_t w = wave - part; w < wave - part + p.unit_waves; w++) {
+            k_top = fmaxf(k_top, s_top[w][0]);
+            v_top = fmaxf(v_top, s_top[w][1]);
+        }
     }
-    const size_t scale_at = size_t(uint32_t(entry)) * p.num_heads_k + head;
-    const uint32_t kept = lo - blk * p.block_size;  // rows in front of the new ones
-    const float k_old = kept ? p.k_scale[scale_at] : 0.0f, v_old = kept ? p.v_scale[scale_at] : 0.0f;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; w++) {
-        k_top = fmaxf(k_top, s_top[0][w]);
-        v_top = fmaxf(v_top, s_top[1][w]);
-    }
+    uint32_t row0;  // pool row of position lo; the block's first row is row0 - kept
+    if (!pool_row(entry, kept, p.block_size, p.num_blocks, &row0) || spare) return;
     const float k_new = fmaxf(k_old, scale_for(k_top)), v_new = fmaxf(v_old, scale_for(v_top));
     const float k_inv = 1.0f / k_new, v_inv = 1.0f / v_new;
-    auto store = [&](uint32_t i, const Quad& k, const Quad& v) {
-        const size_t at = (size_t(row0 + i) * p.num_heads_k + head) * kD + 4 * j;
-        *reinterpret_cast<uint32_t*>(p.k_cache + at) = encode(k, k_inv);
-        *reinterpret_cast<uint32_t*>(p.v_cache + at) = encode(v, v_inv);
+    auto store = [&](uint32_t i, const Oct& k, const Oct& v) {
+        const size_t at = (size_t(row0 + i) * p.num_heads_k + head) * kD + 8 * j;
+        *reinterpret_cast<uint2v*>(p.k_cache + at) = uint2v{encode(k.lo, k_inv), encode(k.hi, k_inv)};
+        *reinterpret_cast<uint2v*>(p.v_cache + at) = uint2v{encode(v.lo, v_inv), encode(v.hi, v_inv)};
     };
 #pragma unroll
-    for (int h = 0; h < kHold; h++) {
-        const uint32_t i = h * stride + wave * kRowsPerPass + sub;
-        if (i < n_rows) store(i, kq[h], vq[h]);
-    }
-    for (uint32_t i = kHold * stride + wave * kRowsPerPass + sub; i < n_rows; i += stride) {
-        Quad k, v;
+    for (int h = 0; h < kHold; h++)
+        if (h * stride + first < n_rows) store(h * stride + first, kq[h], vq[h]);
+    for (uint32_t i = kHold * stride + first; i < n_rows; i += stride) {
+        Oct k, v;
         fetch(i, k, v);
+        turn(i, k);
         store(i, k, v);
     }
     if (k_new > k_old || v_new > v_old) {
-        for (uint32_t i = wave * kRowsPerPass + sub; i < kept; i += stride) {
-            const size_t at = (size_t(row0 - kept + i) * p.num_heads_k + head) * kD + 4 * j;
+        for (uint32_t i = first; i < kept; i += stride) {
+            const size_t at = (size_t(row0 - kept + i) * p.num_heads_k + head) * kD + 8 * j;
             if (k_new > k_old) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(p.k_cache + at);
-                *w = recode(*w, k_old * k_inv);
+                uint2v* w = reinterpret_cast<uint2v*>(p.k_cache + at);
+                *w = uint2v{recode(w->x, k_old * k_inv), recode(w->y, k_old * k_inv)};
             }
             if (v_new > v_old) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(p.v_cache + at);
-                *w = recode(*w, v_old * v_inv);
+                uint2v* w = reinterpret_cast<uint2v*>(p.v_cache + at);
+                *w = uint2v{recode(w->x, v_old * v_inv), recode(w->y, v_old * v_inv)};
             }
         }
-        if (threadIdx.x == 0) {
+        if (part == 0 && lane == 0) {
             p.k_scale[scale_at] = k_new;
             p.v_scale[scale_at] = v_new;
         }
@@ -405,12 +418,16 @@ int launch_rope_append_q8(const granite_hip_rope_q8_args& a) {
         const uint64_t units = a.positions ? uint64_t(a.seq_len)
                                            : uint64_t((end - 1) / a.block_size) - a.start_pos / a.block_size + 1;
         if (units * a.num_heads_k > 0x7FFFFFFFull) return GRANITE_HIP_EINVAL;
-        kv_groups = a.positions ? (units * a.num_heads_k + kWaves - 1) / kWaves : units * a.num_heads_k;
+        p.kv_units = uint32_t(units * a.num_heads_k);
+        const uint32_t held = kHold * (512 / a.head_dim);  // rows a wave holds
+        p.unit_waves = a.block_size <= held ? 1 : a.block_size <= 2 * held ? 2 : 4;
+        const uint32_t per_group = a.positions ? kWaves : kWaves / p.unit_waves;
+        kv_groups = (units * a.num_heads_k + per_group - 1) / per_group;
     }
     if (a.q) {
         const uint64_t octs = uint64_t(a.seq_len) * (a.head_dim / 8) * a.num_heads_q;
         // one head per thread until there are four times as many threads as the part holds at once
-        // (256 CUs x 2048): the lookup of cos and sin is then shared by four heads
+        // (256 CUs x 2048): the lookup of cos and sin is then shared by two heads (8187 tokens: 62.5 us; by four 65)
         p.q_heads = octs >= (2ull << 20) ? kQHeads : 1;
         const uint64_t threads = uint64_t(a.seq_len) * (a.head_dim / 8) * ((a.num_heads_q + p.q_heads - 1) / p.q_heads);
         q_groups = (threads + kThreads - 1) / kThreads;
