@@ -26,7 +26,7 @@
 //
 // V of keys that no row of the workgroup sees is stored as zeros, since 0 * NaN is NaN.  In tiles that only
 // some rows see, infinities and NaNs of V are stored as zeros as well, and where there were any they are added
-// at the end to the rows that see them (add_specials).
+// at the end to the rows that see them.
 #include "common.h"
 #include "kv_attend.h"
 
@@ -606,11 +606,25 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     }
     if (!row_live) return;
     // Accumulator [t][4 a + b] is head-dim element 32 t + 16 (a >> 1) + 8 g + 4 (a & 1) + b: 8 consecutive per (t, a >> 1).
-    if (t_begin < n_tiles && *s_special) {
-        // infinities and NaNs of V that were left out in tiles that not every row sees (rare)
+    bool nan = false;  // infinities of V may have come out as NaN, through a probability's remainder or an underflow to zero
+    if constexpr (!kF8) {
+#pragma unroll
+        for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) nan = nan || oacc[t][r] != oacc[t][r];
+        nan = nan && l_run < INFINITY;
+        if (nan) {
+#pragma unroll
+            for (int t = 0; t < kBlocks; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) oacc[t][r] = oacc[t][r] != oacc[t][r] ? 0.0f : oacc[t][r];
+        }
+    }
+    if (t_begin < n_tiles && (*s_special || nan)) {
+        // the infinities and NaNs of V that were left out in tiles that not every row sees, or all of them (rare)
         for (uint32_t it = t_begin; it < n_tiles; it++) {
             const uint32_t key0 = key_of(it);
-            if (!partial(key0)) continue;
+            if (!nan && !partial(key0)) continue;
             for (uint32_t key = key0; key < min(key0 + kBN, row_hi); key++) {
                 if (key < row_lo && key >= p.sinks) continue;
                 uint32_t at = key;

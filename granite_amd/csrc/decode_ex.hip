@@ -8,14 +8,16 @@
 namespace ghip {
 namespace {
 
-constexpr uint32_t kRowWaves = 4;
+constexpr uint32_t kRowWaves = 8;
 constexpr uint32_t kDirectTokens = 768;
+constexpr uint32_t kStreamRows = 320, kStreamRowsHalf = 160;  // float, half results
 
 // One workgroup per (run of 16 query rows, KV head, sequence, key split).  A row is a (query, head of
 // the KV head's group) pair, row r = query * group + head, so a decode step's group, a few draft tokens and a
 // long chunk are the same thing here.  The waves take the visible tiles in turn and are merged through LDS.
-template <bool kQF32, bool kF8, int kRows, int kD>
-__global__ void __launch_bounds__(kRowWaves* kWave, 1) kv_rows_kernel(KvParams p) {
+// kMulti: several queries, whose rows differ in what they see.
+template <bool kQF32, bool kF8, int kRows, int kD, bool kMulti>
+__global__ void __launch_bounds__(kRowWaves* kWave, 2) kv_rows_kernel(KvParams p) {
     using T = Tile<kF8, kRows, kD>;
     const uint32_t lane = threadIdx.x & 63, wave = ex_uniform(threadIdx.x >> 6);
     const uint32_t n = lane & 15, g = lane >> 4;
@@ -50,12 +52,13 @@ __global__ void __launch_bounds__(kRowWaves* kWave, 1) kv_rows_kernel(KvParams p
         const auto rows = T::rows_from(p, T::entry_of(p, table, tok0, seen, lane), kvh, tok0, seen, lane);
         tile.load(p, rows, kvh, lane);
         const bool masked = T::needs_mask(p, rows, tok0, lo_all, hi_all);
-        attend_tile<kQF32, kF8, kRows, kD, true>(p, tile, rows, tok0, seen, lo, hi, masked, st, lane);
+        attend_tile<kQF32, kF8, kRows, kD, kMulti>(p, tile, rows, tok0, seen, lo, hi, masked, st, lane);
     }
 
     // ---- the waves' results, combined through LDS
     __shared__ float s_ml[kRowWaves][16][2];
-    __shared__ float s_o[kRowWaves][16][kD + 4];
+    extern __shared__ float s_o_raw[];  // [kRowWaves][16][kD + 4]
+    auto s_o = [&](uint32_t w, uint32_t row, uint32_t d) __attribute__((always_inline)) -> float& { return s_o_raw[(w * 16 + row) * (kD + 4) + d]; };
     {
         float l = st.l;
         l += wave_shfl_xor(l, 16);
@@ -67,7 +70,7 @@ __global__ void __launch_bounds__(kRowWaves* kWave, 1) kv_rows_kernel(KvParams p
         const float unit = st.vref * (1.0f / kExBoost);
         if (32 * g < uint32_t(kD)) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) s_o[wave][n][32 * g + e] = st.acc[e & 7][e >> 3] * unit;
+            for (int e = 0; e < 32; e++) s_o(wave, n, 32 * g + e) = st.acc[e & 7][e >> 3] * unit;
         }
     }
     __syncthreads();
@@ -82,7 +85,7 @@ __global__ void __launch_bounds__(kRowWaves* kWave, 1) kv_rows_kernel(KvParams p
         for (uint32_t w = 0; w < kRowWaves; w++) {
             const float f = fast_exp2(s_ml[w][row][0] - m);
             l += s_ml[w][row][1] * f;
-            o += s_o[w][row][d] * f;
+            o += s_o(w, row, d) * f;
         }
         const uint32_t q = (rt * 16 + row) / p.group, h = kvh * p.group + (rt * 16 + row) % p.group;
         if (p.n_splits > 1) {
@@ -94,7 +97,7 @@ __global__ void __launch_bounds__(kRowWaves* kWave, 1) kv_rows_kernel(KvParams p
             }
             continue;
         }
-        const float result = l > 0.0f ? o / l : l == 0.0f ? 0.0f : l;  // (l NaN: the row is NaN)
+        const float result = settle_nan(p, l == 0.0f ? 0.0f : o / l, l, b, kvh, start + q, len, d);
         const int64_t at = int64_t(b) * p.out_batch + int64_t(q) * p.out_tok + int64_t(h) * p.out_head + d;
         if (p.out_f32) static_cast<float*>(p.out)[at] = result;
         else static_cast<_Float16*>(p.out)[at] = static_cast<_Float16>(result);
@@ -117,7 +120,8 @@ __global__ void kv_rows_merge_kernel(KvParams p, uint32_t D) {
         l += p.part_ml[(row + s * step) * 2 + 1] * f;
         o += p.part_o[(row + s * step) * D + d] * f;
     }
-    const float result = l > 0.0f ? o / l : l == 0.0f ? 0.0f : l;
+    const uint32_t len = p.decode ? ex_seq_len(p, b) : p.max_tokens;
+    const float result = settle_nan(p, l == 0.0f ? 0.0f : o / l, l, b, h / p.group, p.decode ? len - 1 : p.start_pos + q, len, d);
     const int64_t at = int64_t(b) * p.out_batch + int64_t(q) * p.out_tok + int64_t(h) * p.out_head + d;
     if (p.out_f32) static_cast<float*>(p.out)[at] = result;
     else static_cast<_Float16*>(p.out)[at] = static_cast<_Float16>(result);
@@ -126,20 +130,29 @@ __global__ void kv_rows_merge_kernel(KvParams p, uint32_t D) {
             l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kExLn2;
 }
 
+template <bool kQF32, bool kF8, int kRows, int kD, bool kMulti>
+int launch_rows_one(const KvParams& p, dim3 grid) {
+    auto kernel = kv_rows_kernel<kQF32, kF8, kRows, kD, kMulti>;
+    constexpr size_t kLds = size_t(kRowWaves) * 16 * (kD + 4) * sizeof(float);
+    static bool configured[kMaxDevices];
+    if (int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(kernel), kLds, configured)) return rc;
+    kernel<<<grid, dim3(kRowWaves * kWave), kLds, ctx().stream>>>(p);
+    return launch_status();
+}
 template <bool kQF32, bool kF8, int kRows>
-void launch_rows_dim(const KvParams& p, dim3 grid, uint32_t D) {
-    const dim3 block(kRowWaves * kWave);
-    if (D == 128) kv_rows_kernel<kQF32, kF8, kRows, 128><<<grid, block, 0, ctx().stream>>>(p);
-    else kv_rows_kernel<kQF32, kF8, kRows, 64><<<grid, block, 0, ctx().stream>>>(p);
+int launch_rows_dim(const KvParams& p, dim3 grid, uint32_t D) {
+    if (p.decode)
+        return D == 128 ? launch_rows_one<kQF32, kF8, kRows, 128, false>(p, grid) : launch_rows_one<kQF32, kF8, kRows, 64, false>(p, grid);
+    return D == 128 ? launch_rows_one<kQF32, kF8, kRows, 128, true>(p, grid) : launch_rows_one<kQF32, kF8, kRows, 64, true>(p, grid);
 }
 
 template <bool kQF32>
-void launch_rows_cache(const KvParams& p, dim3 grid, uint32_t D, bool f8, int rows) {
-    if (f8 && rows == kExPaged16) launch_rows_dim<kQF32, true, kExPaged16>(p, grid, D);
-    else if (f8) launch_rows_dim<kQF32, true, kExPagedAny>(p, grid, D);
-    else if (rows == kExContiguous) launch_rows_dim<kQF32, false, kExContiguous>(p, grid, D);
-    else if (rows == kExPaged16) launch_rows_dim<kQF32, false, kExPaged16>(p, grid, D);
-    else launch_rows_dim<kQF32, false, kExPagedAny>(p, grid, D);
+int launch_rows_cache(const KvParams& p, dim3 grid, uint32_t D, bool f8, int rows) {
+    if (f8 && rows == kExPaged16) return launch_rows_dim<kQF32, true, kExPaged16>(p, grid, D);
+    if (f8) return launch_rows_dim<kQF32, true, kExPagedAny>(p, grid, D);
+    if (rows == kExContiguous) return launch_rows_dim<kQF32, false, kExContiguous>(p, grid, D);
+    if (rows == kExPaged16) return launch_rows_dim<kQF32, false, kExPaged16>(p, grid, D);
+    return launch_rows_dim<kQF32, false, kExPagedAny>(p, grid, D);
 }
 
 // The row kernel for any launch.
@@ -152,7 +165,7 @@ int launch_rows(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const Scr
     const uint32_t keys = p.window ? uint32_t(min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks)) : p.max_tokens;
     const uint32_t tiles = (keys + 63) / 64;
     uint32_t splits = wgs < cus ? uint32_t((cus + wgs - 1) / wgs) : 1u;
-    splits = min(splits, max(tiles / (2 * kRowWaves), 1u));
+    splits = min(splits, max(tiles / kRowWaves, 1u));
     p.n_splits = min(splits, 64u);
     if (uint64_t(row_tiles) * p.n_splits > 0x7FFFFFFFull) return GRANITE_HIP_EINVAL;
     const size_t slots = p.n_splits > 1 ? size_t(p.n_splits) * p.batch * p.num_heads * p.seq_q : 0;
@@ -168,13 +181,12 @@ int launch_rows(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const Scr
         p.part_o = static_cast<float*>(ws);
         p.part_ml = p.part_o + slots * D;
     }
+    int rc;
     {
         KernelTimerScope timer(p.decode ? "decode_ex" : "attention_ex");
         const dim3 grid(row_tiles * p.n_splits, p.num_kv_heads, p.batch);
-        if (q_f32) launch_rows_cache<true>(p, grid, D, f8, rows);
-        else launch_rows_cache<false>(p, grid, D, f8, rows);
+        rc = q_f32 ? launch_rows_cache<true>(p, grid, D, f8, rows) : launch_rows_cache<false>(p, grid, D, f8, rows);
     }
-    int rc = launch_status();
     if (rc != GRANITE_HIP_OK || p.n_splits == 1) return rc;
     {
         KernelTimerScope timer(p.decode ? "decode_ex_merge" : "attention_ex_merge");
@@ -332,6 +344,14 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     p.causal = a.mask_mode == GRANITE_HIP_MASK_CAUSAL;
     p.start_pos = a.start_pos;
     p.scale_log2 = a.scale * kExLog2e;
+    // Few rows of 8-bit pools: the persistent kernel of the decode step, 16 rows in the place of a head's group
+    const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3;
+    if (f8 && rows == kExPaged16 && uint64_t(a.seq_q) * p.group <= (p.out_f32 ? kStreamRows : kStreamRowsHalf)) {
+        const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
+        const uint32_t tiles = uint32_t((seen + 31) / 32);
+        p.q_groups = uint32_t((uint64_t(a.seq_q) * p.group + 15) / 16);
+        if (kv_stream_supports(p, tiles)) return launch_kv_stream(p, D, a.q_dtype == GRANITE_HIP_F32, f8, rows, tiles, scratch);
+    }
     if (rows != kExPagedAny && uint64_t(a.seq_q) * p.group > 32)
         return launch_kv_tiles(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
     return launch_rows(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);

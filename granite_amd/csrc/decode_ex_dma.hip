@@ -59,7 +59,10 @@ struct Geo {
     }
 };
 
-template <bool kQF32, int kD, uint32_t kPer>
+// kMulti: several queries of one sequence.  The rows of a KV head, row = query * group + head, take the place of its group's
+// heads: 16 of them are a "head" of the list, which streams the KV head's tiles as any other (few rows: what they share
+// they find in the L2).
+template <bool kQF32, int kD, uint32_t kPer, bool kMulti>
 __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
     using G = Geo<kD>;
     constexpr int kSteps = kD / 32, kBlocks = kD / 16;
@@ -77,7 +80,11 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
     // ---- tile counts and their prefix sums, as in decode_ex_stream.hip
     __shared__ uint32_t s_wave_sum[kWaves];
     const uint32_t vheads = p.num_kv_heads * p.q_groups;
-    auto seen_of = [&](uint32_t len) __attribute__((always_inline)) { return visible_tiles<kTokens>(len - 1, len, p.window, p.sinks); };
+    const uint32_t n_rows = kMulti ? p.seq_q * p.group : p.group;  // of a KV head
+    auto seen_of = [&](uint32_t len) __attribute__((always_inline)) {
+        if constexpr (kMulti) return visible_tiles<kTokens>(p.start_pos, p.causal ? min(len, p.start_pos + p.seq_q) : len, p.window, p.sinks);
+        else return visible_tiles<kTokens>(len - 1, len, p.window, p.sinks);
+    };
     auto count_of = [&](uint32_t len) __attribute__((always_inline)) { return len ? seen_of(len).count : 0u; };
     uint32_t tiles_total;
     {
@@ -175,8 +182,9 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
     };
     // step 3, the scales being there.  A run that no query sees has scale 0, whatever lies in the arrays.
     auto plan_scales = [&](Plan& q) __attribute__((always_inline)) {
-        const uint32_t first = run_token(q), lo = window_begin(max(q.len, 1u) - 1, p.window);
-        const bool used = bool(int(q.valid) & int(first < q.len) & (int(first + 15 >= lo) | int(first < p.sinks)));
+        const VisibleTiles seen = seen_of(max(q.len, 1u));
+        const uint32_t first = run_token(q), lo = seen.lo;
+        const bool used = bool(int(q.valid) & int(first < seen.end) & (int(first + 15 >= lo) | int(first < p.sinks)));
         const float ks = reinterpret_cast<const float*>(s_side)[64 + lane], vs = reinterpret_cast<const float*>(s_side)[128 + lane];
         q.ks = used ? ks : 0.0f;
         q.vs = used ? vs : 0.0f;
@@ -245,10 +253,27 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
 #pragma unroll
         for (int t = 0; t < kBlocks; t++) acc[t] = float4v{0, 0, 0, 0};
     };
+    // what the lane's row sees: keys in front of row_hi, from row_lo on or sinks; every row of the wave sees those in front of
+    // all_hi, from all_lo on
+    uint32_t row_hi = 0, row_lo = 0, all_hi = 0, all_lo = 0;
     auto load_q = [&](const Unit& u) __attribute__((always_inline)) {
-        const uint32_t vh = (u.lh & 0x7FFFFFFFu) * kPer + wave % kPer, kvh = vh / p.q_groups, in_group = (vh % p.q_groups) * 16 + n;
-        const bool live = in_group < p.group;
-        const int64_t at = int64_t(u.b) * p.q_batch + int64_t(kvh * p.group + (live ? in_group : 0)) * p.q_head;
+        const uint32_t vh = (u.lh & 0x7FFFFFFFu) * kPer + wave % kPer, kvh = vh / p.q_groups, row0 = (vh % p.q_groups) * 16;
+        const bool live = row0 + n < n_rows;
+        const uint32_t row = live ? row0 + n : row0;
+        int64_t at = int64_t(u.b) * p.q_batch;
+        if constexpr (kMulti) {
+            const uint32_t query = row / p.group, last = (min(row0 + 16, n_rows) - 1) / p.group;
+            at += int64_t(query) * p.q_tok + int64_t(kvh * p.group + (row - query * p.group)) * p.q_head;
+            auto limit = [&](uint32_t pos) __attribute__((always_inline)) { return p.causal ? min(u.len, pos + 1) : u.len; };
+            row_hi = limit(p.start_pos + query);
+            row_lo = window_begin(p.start_pos + query, p.window);
+            all_hi = limit(p.start_pos + row0 / p.group);
+            all_lo = window_begin(p.start_pos + last, p.window);
+        } else {
+            at += int64_t(kvh * p.group + row) * p.q_head;
+            row_hi = all_hi = u.len;
+            row_lo = all_lo = window_begin(u.len - 1, p.window);
+        }
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
             const int64_t off = at + 64 * (s / 2) + 16 * g + 8 * (s % 2);
@@ -277,13 +302,10 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
         float l = l_run;
         l += wave_shfl_xor(l, 16);
         l += wave_shfl_xor(l, 32);
-        const uint32_t lh = u.lh & 0x7FFFFFFFu;
-        const uint32_t vh = lh * kPer + wave % kPer, kvh = vh / p.q_groups, in_group = (vh % p.q_groups) * 16 + n;
-        if (in_group < p.group) {
-            const uint32_t v0 = lh * kPer;
-            const uint32_t first_head = (v0 / p.q_groups) * p.group + (v0 % p.q_groups) * 16;
+        const uint32_t lh = u.lh & 0x7FFFFFFFu, row0 = ((lh * kPer + wave % kPer) % p.q_groups) * 16;
+        if (row0 + n < n_rows) {
             const uint32_t piece = worker + u.b * lists + lh;
-            const size_t at = size_t(piece) * p.part_cap + (kvh * p.group + in_group - first_head);
+            const size_t at = size_t(piece) * p.part_cap + (wave % kPer) * (p.part_cap / kPer) + n;
             const float unit = vref * (1.0f / kExBoost);
 #pragma unroll
             for (int t = 0; t < kBlocks; t++) *reinterpret_cast<float4v*>(p.part_o + at * kD + 16 * t + 4 * g) = acc[t] * unit;
@@ -339,19 +361,24 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
         for (int sub = 0; sub < 2; sub++)
 #pragma unroll
             for (int i = 0; i < 4; i++) s[sub][i] = c[sub][i] * (u.ks[sub] * p.scale_log2);
-        const uint32_t lo = window_begin(u.len - 1, p.window);
-        if (u.tok + kTokens > u.len || (u.tok < lo && u.tok + kTokens > p.sinks) || u.valid != 3) {
+        uint32_t sees = 0xFFu;  // kMulti: bit 4 sub + i, the lane's row sees token 16 sub + 4 g + i
+        const bool masked = u.tok + kTokens > all_hi || (u.tok < all_lo && u.tok + kTokens > p.sinks) || u.valid != 3;
+        if (masked) {
             uint32_t keep[2];  // a byte per token
+            if constexpr (kMulti) sees = 0;
+            const VisibleTiles seen = seen_of(u.len);
 #pragma unroll
             for (int sub = 0; sub < 2; sub++) {
                 keep[sub] = 0;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const uint32_t tok = u.tok + 16 * sub + 4 * g + i;
-                    const bool vis = bool(int((u.valid >> sub) & 1u) & int(tok < u.len) & (int(tok >= lo) | int(tok < p.sinks)));
+                    const uint32_t tok = u.tok + 16 * sub + 4 * g + i, valid = (u.valid >> sub) & 1u;
+                    const bool vis = bool(int(valid) & int(tok < row_hi) & (int(tok >= row_lo) | int(tok < p.sinks)));
+                    const bool any = kMulti ? bool(int(valid) & int(tok < seen.end) & (int(tok >= seen.lo) | int(tok < p.sinks))) : vis;
                     s[sub][i] = vis ? s[sub][i] : -INFINITY;
-                    keep[sub] |= vis ? 0xFFu << (8 * i) : 0u;
-                    asm volatile("" : "+v"(s[sub][i]), "+v"(keep[sub]));
+                    keep[sub] |= any ? 0xFFu << (8 * i) : 0u;
+                    if constexpr (kMulti) sees |= vis ? 1u << (4 * sub + i) : 0u;
+                    asm volatile("" : "+v"(s[sub][i]), "+v"(keep[sub]), "+v"(sees));
                 }
             }
 #pragma unroll
@@ -391,6 +418,27 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
                 const _Float16 h = static_cast<_Float16>(scaled);
                 hi[4 * sub + i] = h;
                 rem[4 * sub + i] = static_cast<_Float16>(scaled - static_cast<float>(h));
+            }
+        }
+        if (kMulti && masked) {
+            // a NaN of V reaches the rows that see its token and no others: taken out of V, and put back through a product
+            // of "is NaN" and "sees"
+            half8 see;
+#pragma unroll
+            for (int j = 0; j < 8; j++) see[j] = (sees >> j) & 1u ? _Float16(1) : _Float16(0);
+#pragma unroll
+            for (int t = 0; t < kBlocks; t++) {
+                uint2v nan;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    // bytes whose low seven bits are all ones: adding one carries into bit 7
+                    const uint32_t hit = ((vw[t][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    vw[t][w] &= ~((hit >> 7) * 0xFFu);
+                    nan[w] = (hit >> 7) * 0x38u;  // 1.0
+                }
+                const float4v mark = __builtin_amdgcn_mfma_f32_16x16x32_f16(f8x8_to_half8(nan.x, nan.y), see, float4v{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[t][i] = mark[i] > 0.0f ? NAN : acc[t][i];
             }
         }
 #pragma unroll
@@ -437,13 +485,17 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
     }
 }
 
-template <bool kQF32, int kD, uint32_t kPer>
-int launch_per(const KvParams& p, dim3 grid, size_t lds) {
-    auto kernel = kv_dma_kernel<kQF32, kD, kPer>;
+template <bool kQF32, int kD, uint32_t kPer, bool kMulti>
+int launch_rows_of(const KvParams& p, dim3 grid, size_t lds) {
+    auto kernel = kv_dma_kernel<kQF32, kD, kPer, kMulti>;
     static bool configured[kMaxDevices];
     if (int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(kernel), kv_dma_lds_bytes(kD, kDmaMaxBatch), configured)) return rc;
     kernel<<<grid, dim3(kWaves * kWave), lds, ctx().stream>>>(p);
     return launch_status();
+}
+template <bool kQF32, int kD, uint32_t kPer>
+int launch_per(const KvParams& p, dim3 grid, size_t lds) {
+    return p.decode ? launch_rows_of<kQF32, kD, kPer, false>(p, grid, lds) : launch_rows_of<kQF32, kD, kPer, true>(p, grid, lds);
 }
 template <bool kQF32, int kD>
 int launch_d(const KvParams& p, uint32_t per_list, dim3 grid, size_t lds) {

@@ -28,12 +28,6 @@ constexpr uint32_t kWaves = 8;
 constexpr uint32_t kPlanHeader = 4;
 constexpr uint32_t kMaxPrefix = 7680;  // lengths and prefix sums in LDS: 60 KiB
 
-// First query head of list head `lh`.
-__device__ __forceinline__ uint32_t first_query_head(const KvParams& p, uint32_t lh, uint32_t per_list) {
-    const uint32_t v0 = lh * per_list;
-    return (v0 / p.q_groups) * p.group + (v0 % p.q_groups) * 16;
-}
-
 template <bool kQF32, bool kF8, int kRows, int kD, uint32_t kPer>
 __global__ void __launch_bounds__(kWaves* kWave, 2) kv_stream_kernel(KvParams p) {
     using T = Tile<kF8, kRows, kD>;
@@ -145,11 +139,10 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_stream_kernel(KvParams p)
         float l = st.l;
         l += wave_shfl_xor(l, 16);
         l += wave_shfl_xor(l, 32);
-        const uint32_t kvh = vh / p.q_groups, in_group = (vh % p.q_groups) * 16 + n;
+        const uint32_t in_group = (vh % p.q_groups) * 16 + n;
         if (in_group < p.group && 32 * g < uint32_t(kD)) {
             const uint32_t piece = worker + of_unit(d_b, i) * lists + lh;
-            const uint32_t local = kvh * p.group + in_group - first_query_head(p, lh, kPer);
-            const size_t at = size_t(piece) * p.part_cap + local;
+            const size_t at = size_t(piece) * p.part_cap + (wave % kPer) * (p.part_cap / kPer) + n;
             float* po = p.part_o + at * kD + 32 * g;
             const float unit = st.vref * (1.0f / kExBoost);
 #pragma unroll
@@ -206,22 +199,24 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_stream_kernel(KvParams p)
     }
 }
 
-// Joins the pieces of one (sequence, query head): the workers that touched its list head are consecutive.  kJoin
+// Joins the pieces of one (sequence, row): the workers that touched its list head are consecutive.  kJoin
 // groups of threads take four pieces at a time in turn and are joined through LDS: 4 where sequences are few (a long
 // one alone has a piece of every worker: 2 sequences of 131072 tokens 17.5 -> 7.3 us), 1 where they are many and short
 // of pieces (64 sequences: 5.3 us against 6.8).
 template <int kD, uint32_t kJoin>
 __global__ void __launch_bounds__(kD* kJoin) kv_stream_merge_kernel(KvParams p) {
-    const uint32_t qh = blockIdx.x, b = blockIdx.y, d = threadIdx.x % kD, part = threadIdx.x / kD;
+    const uint32_t n_rows = p.seq_q * p.group;  // of a KV head: (query, head of the group) pairs
+    const uint32_t kvh = blockIdx.x / n_rows, row = blockIdx.x - kvh * n_rows;
+    const uint32_t b = blockIdx.y, d = threadIdx.x % kD, part = threadIdx.x / kD;
     const uint32_t* prefix = p.plan + kPlanHeader;
     const uint32_t nt = prefix[b + 1] - prefix[b];
     if (nt == 0) return;  // empty sequence: its output stays
     const uint32_t per = p.plan[0], per_list = p.plan[1];
     const uint32_t lists = p.num_kv_heads * p.q_groups / per_list;
-    const uint32_t lh = ((qh / p.group) * p.q_groups + (qh % p.group) / 16) / per_list;
+    const uint32_t vh = kvh * p.q_groups + row / 16, lh = vh / per_list;
     const uint32_t u_start = prefix[b] * lists + lh * nt;
     const uint32_t first_worker = u_start / per, n_parts = (u_start + nt - 1) / per - first_worker + 1;
-    const size_t at0 = size_t(first_worker + b * lists + lh) * p.part_cap + (qh - first_query_head(p, lh, per_list));
+    const size_t at0 = size_t(first_worker + b * lists + lh) * p.part_cap + (vh % per_list) * (p.part_cap / per_list) + row % 16;
     float mx = kExNegBig, o = 0.0f, l = 0.0f;
     for (uint32_t c0 = 4 * part; c0 < n_parts; c0 += 4 * kJoin) {  // four at a time: their loads are in flight together
         float m[4], ls[4], os[4];
@@ -266,9 +261,15 @@ __global__ void __launch_bounds__(kD* kJoin) kv_stream_merge_kernel(KvParams p) 
     } else if (part != 0) {
         return;
     }
-    static_cast<float*>(p.out)[int64_t(b) * p.out_batch + int64_t(qh) * p.out_head + d] = l == 0.0f ? 0.0f : o / l;
+    const uint32_t query = row / p.group, head = kvh * p.group + (row - query * p.group);
+    const int64_t at = int64_t(b) * p.out_batch + int64_t(query) * p.out_tok + int64_t(head) * p.out_head + d;
+    const uint32_t len = ex_seq_len(p, b);
+    const float result = settle_nan(p, l == 0.0f ? 0.0f : o / l, l, b, kvh, p.decode ? len - 1 : p.start_pos + query, len, d);
+    if (p.out_f32) static_cast<float*>(p.out)[at] = result;
+    else static_cast<_Float16*>(p.out)[at] = static_cast<_Float16>(result);
     if (p.lse && d == 0)
-        p.lse[int64_t(b) * p.lse_batch + int64_t(qh) * p.lse_head] = l == 0.0f ? -INFINITY : (mx + __builtin_amdgcn_logf(l)) * kExLn2;
+        p.lse[int64_t(b) * p.lse_batch + int64_t(query) * p.lse_tok + int64_t(head) * p.lse_head] =
+            l == 0.0f ? -INFINITY : (mx + __builtin_amdgcn_logf(l)) * kExLn2;
 }
 
 template <bool kQF32, bool kF8, int kRows, int kD>
@@ -309,7 +310,7 @@ int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint
     p.workers = cus * (kWaves / per_list);
     // smallest range of a worker: a short batch is not cut into ranges of a tile or two, each with a partial to join
     p.min_per = max(1u, min(4u, (tiles_per_seq + 31) / 32));
-    p.part_cap = per_list * min(p.group, 16u);
+    p.part_cap = per_list * min(p.seq_q * p.group, 16u);
     const size_t slots = (size_t(p.workers) + size_t(p.batch) * lists) * p.part_cap;
     const size_t plan_bytes = ((kPlanHeader + size_t(p.batch) + 1) * sizeof(uint32_t) + 255) & ~size_t(255);
     const size_t need = plan_bytes + slots * (D + 2) * sizeof(float);
@@ -339,7 +340,7 @@ int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint
     if (int rc = launch_status()) return rc;
     {
         KernelTimerScope timer("decode_ex_merge");
-        const dim3 grid(p.num_heads, p.batch);
+        const dim3 grid(p.seq_q * p.num_heads, p.batch);
         const bool few = size_t(p.batch) * lists * 16 <= p.workers;  // 16 pieces a segment or more if all are as long
         hipStream_t st = ctx().stream;
         if (D == 128 && few) kv_stream_merge_kernel<128, 4><<<grid, dim3(512), 0, st>>>(p);

@@ -350,6 +350,29 @@ struct Rows16 {
     }
 };
 
+// The output element d of a row whose sum came out as NaN although its probabilities did not: with infinities among the V it
+// sees of a half cache the products of a probability's half and remainder may cancel (inf - inf) or vanish (inf * 0) where the
+// sum is infinite.  It is the sum of the infinities and NaNs the row sees.  (Not for 8-bit pools, whose only special is NaN.)
+__device__ __forceinline__ float settle_nan(const KvParams& p, float result, float l, uint32_t b, uint32_t kvh, uint32_t pos, uint32_t len, uint32_t d) {
+    if (result == result || p.k_scale || !(l < INFINITY)) return result;
+    const uint32_t lo = window_begin(pos, p.window), hi = p.causal ? min(len, pos + 1) : len;
+    float sum = 0.0f;
+    for (uint32_t key = 0; key < hi; key++) {
+        if (key < lo && key >= p.sinks) {
+            key = lo - 1;
+            continue;
+        }
+        uint32_t row = key;
+        if (p.tables) {
+            const uint32_t blk = key / p.block_size;
+            if (!pool_row(p.tables[size_t(b) * p.max_blocks + blk], key - blk * p.block_size, p.block_size, p.num_blocks, &row)) continue;
+        }
+        const float x = static_cast<float>(reinterpret_cast<const _Float16*>(p.v + int64_t(kvh) * p.head_bytes + int64_t(row) * p.row_bytes)[d]);
+        if (!(fabsf(x) < INFINITY)) sum += x;
+    }
+    return sum != 0.0f ? sum : result;
+}
+
 // The maximum over the four lanes n, n + 16, n + 32, n + 48, in all of them: two register swaps, no LDS round trip
 // (v_permlane16_swap exchanges the odd rows of 16 lanes of one register with the even rows of the other).
 __device__ __forceinline__ float max_over_groups(float v) {
@@ -393,6 +416,7 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
 #pragma unroll
         for (int i = 0; i < 4; i++) s[sub][i] = c[i] * (kF8 ? of_token(rows.ks, sub, i) * p.scale_log2 : p.scale_log2);
     }
+    bool special = false;  // kPerRow, masked: some V of the tile is infinite or NaN
     uint32_t visible = 0xFFFFu;  // bit 4 sub + i: the lane's row sees token 16 sub + 4 g + i
     if (masked) {
         if constexpr (kPerRow) visible = 0;
@@ -417,6 +441,19 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
                     asm volatile("" : "+v"(tile.vr[4 * sub + i][w]));
                 }
             }
+        if constexpr (kPerRow) {
+            uint32_t hit = 0;
+#pragma unroll
+            for (int j = 0; j < 4 * kSubs; j++)
+#pragma unroll
+                for (int w = 0; w < T::kVWords; w++) {
+                    // 8 bits: a byte's low seven bits are all ones; half: its exponent's five are.  Adding one in the lowest
+                    // place of those carries into the bit above.
+                    const uint32_t x = tile.vr[j][w];
+                    hit |= kF8 ? ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u : ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                }
+            special = __any(hit != 0);
+        }
     }
     float top = s[0][0];
 #pragma unroll
@@ -462,7 +499,7 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
 #pragma unroll
         for (int w = 0; w < T::kVWords; w++)
             tile.v_operands(pair, w, [&](int t, half8 a) __attribute__((always_inline)) {
-                if (kPerRow && masked) {
+                if (kPerRow && special) {
                     half8 plus, minus, sees;
 #pragma unroll
                     for (int j = 0; j < 8; j++) {

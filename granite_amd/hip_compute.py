@@ -67,8 +67,8 @@ class DeviceBuffer:
 
 
 def _p(buf) -> Optional[int]:
-    if buf is None:
-        return None
+    if buf is None or type(buf) is int:
+        return buf
     return buf.ptr if isinstance(buf, DeviceBuffer) else int(buf)
 
 

@@ -256,6 +256,23 @@ def test_nan_where_it_is_seen(gpu):
     assert np.isposinf(got[0, :, 5]).all() and np.isfinite(np.delete(got, 5, -1)).all()
 
 
+def test_infinities_that_are_seen(gpu):
+    """An infinity anywhere in what a row sees makes its sum infinite, whatever the probability's rounding."""
+    for bs, lens in ((16, [2000, 90]), (20, [2000, 90]), (16, [300])):
+        cache = Cache(np.random.default_rng(21), lens, bs, 2, 64, F16)
+        at = lambda t: cache.table[0, t // bs] * bs + t % bs  # noqa: E731
+        n = lens[0]
+        cache.v[at(n - 1), 0, 3] = cache.v[at(n - 60), 0, 4] = np.inf
+        cache.v[at(n - 40), 1, 5] = -np.inf
+        cache.v[at(n - 41), 1, 6], cache.v[at(n - 42), 1, 6] = np.inf, -np.inf
+        cache.upload()
+        got, _ = run_decode(gpu, cache, 4, F16, n - 7, 2)
+        assert np.isposinf(got[0, :2, 3:5]).all() and np.isneginf(got[0, 2:, 5]).all() and np.isnan(got[0, 2:, 6]).all()
+        for q, o in ((F16, F16), (F32, F32)):
+            for rows in (5, 130):
+                run_prefill(gpu, cache, rows, n - rows, 4, q, o, n - 7, 2, cache_len=n, scale=0.02)
+
+
 # ------------------------------------------------------------------ several queries
 
 @pytest.mark.parametrize("n,start,bs,hq,hkv,d", [
