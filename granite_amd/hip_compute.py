@@ -72,6 +72,11 @@ def _p(buf) -> Optional[int]:
     return buf.ptr if isinstance(buf, DeviceBuffer) else int(buf)
 
 
+def _ptrs(*bufs) -> list:
+    """_p of each: one call where a launch of a few microseconds has a dozen pointers."""
+    return [b if b is None or type(b) is int else _p(b) for b in bufs]
+
+
 class HipCompute:
     """One in-order queue of attention / KV work on one MI355X."""
 
@@ -282,10 +287,12 @@ class HipCompute:
         """decode_attention over a cache of kv_dtype (F8E4M3: paged, with k_scale / v_scale
         [num_blocks, num_kv_heads]), each query seeing the last `window` tokens (0: all) and the
         first num_sinks."""
-        a = DecodeArgs(_p(q), q_dtype, _p(k_cache), _p(v_cache), _p(block_tables), _p(seq_lens), _p(out), _p(lse),
-                       batch_size, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, max_seq,
-                       scale, fixed_seq_len, 0)
-        f = KvForm(kv_dtype, _p(k_scale), _p(v_scale), num_blocks, window, num_sinks)
+        q, k_cache, v_cache, block_tables, seq_lens, out, lse, k_scale, v_scale = _ptrs(
+            q, k_cache, v_cache, block_tables, seq_lens, out, lse, k_scale, v_scale)
+        a = DecodeArgs(q, q_dtype, k_cache, v_cache, block_tables, seq_lens, out, lse, batch_size,
+                       num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, max_seq, scale,
+                       fixed_seq_len, 0)
+        f = KvForm(kv_dtype, k_scale, v_scale, num_blocks, window, num_sinks)
         if query_workspace:
             need = C.c_size_t()
             check(self.lib.granite_hip_decode_ex_workspace_required(C.byref(a), C.byref(f), C.byref(need)),
@@ -301,11 +308,12 @@ class HipCompute:
                      workspace_bytes=None, query_workspace=False):
         """attention over a cache of kv_dtype, with the window of decode_attention_ex at every query's
         position start_pos + index."""
-        a = AttentionArgs(_p(q), q_dtype, q_tok_stride, q_head_stride, _p(out), out_dtype, out_tok_stride,
-                          out_head_stride, _p(lse), _p(k_cache), _p(v_cache), _p(block_table), block_size, max_seq,
-                          cache_len, None, None, 0, None, mask_mode, start_pos, seq_q, num_heads, num_kv_heads,
+        q, out, lse, k_cache, v_cache, block_table, k_scale, v_scale = _ptrs(
+            q, out, lse, k_cache, v_cache, block_table, k_scale, v_scale)
+        a = AttentionArgs(q, q_dtype, q_tok_stride, q_head_stride, out, out_dtype, out_tok_stride, out_head_stride,
+                          lse, k_cache, v_cache, block_table, block_size, max_seq, cache_len, None, None, 0, None, mask_mode, start_pos, seq_q, num_heads, num_kv_heads,
                           head_dim, scale)
-        f = KvForm(kv_dtype, _p(k_scale), _p(v_scale), num_blocks, window, num_sinks)
+        f = KvForm(kv_dtype, k_scale, v_scale, num_blocks, window, num_sinks)
         if query_workspace:
             need = C.c_size_t()
             check(self.lib.granite_hip_attention_ex_workspace_required(C.byref(a), C.byref(f), C.byref(need)),
@@ -321,10 +329,11 @@ class HipCompute:
                        freq_base=10000.0) -> None:
         """rope_append into 8-bit pools with a scale per (block, KV head): Q rotated into q_out, K
         (rotated) and V appended as e4m3 codes."""
-        a = RopeQ8Args(_p(q), _p(q_out), _p(k), _p(v), src_dtype, q_out_dtype, _p(k_cache), _p(v_cache), _p(k_scale),
-                       _p(v_scale), _p(block_table), _p(cos_table), _p(sin_table), table_positions, freq_base,
-                       num_heads_q, num_heads_k, seq_len, head_dim, start_pos, block_size, num_blocks,
-                       max_blocks_per_seq, _p(positions), table_stride)
+        q, q_out, k, v, k_cache, v_cache, k_scale, v_scale, block_table, cos_table, sin_table, positions = _ptrs(
+            q, q_out, k, v, k_cache, v_cache, k_scale, v_scale, block_table, cos_table, sin_table, positions)
+        a = RopeQ8Args(q, q_out, k, v, src_dtype, q_out_dtype, k_cache, v_cache, k_scale, v_scale, block_table,
+                       cos_table, sin_table, table_positions, freq_base, num_heads_q, num_heads_k, seq_len,
+                       head_dim, start_pos, block_size, num_blocks, max_blocks_per_seq, positions, table_stride)
         check(self.lib.granite_hip_rope_append_q8(C.byref(a)), "rope_append_q8")
 
     # ---- scratch memory
