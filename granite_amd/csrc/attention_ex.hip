@@ -11,7 +11,7 @@
 //   window + 256 / group keys for rows that see `window` each (with a head to itself it would visit window + 256), and
 //   a chunk of 37 queries in groups of 4 is one workgroup's worth of rows instead of four quarter-full ones.
 // * Codes become halves once per workgroup, on the way from registers to LDS (v_cvt_scalef32_pk_f16_fp8,
-//   two a cycle and lane): a half holds every e4m3 value, so the products are those of the codes themselves.  Converting
+//   two codes an instruction): a half holds every e4m3 value, so the products are those of the codes themselves.  Converting
 //   operands as they are read would put four conversions beside every MFMA of every wave.
 // * Scales never touch an element of K or V.  A run of 16 keys lies in one block (block sizes are multiples of
 //   16 here), so a sub-tile has two scales of K and two of V.  K's goes into the factor that takes a score to the
@@ -37,6 +37,7 @@ constexpr int kBM = 256;  // query rows per workgroup
 constexpr int kBN = 64;   // keys per tile
 constexpr int kThreads = 512;
 constexpr int kKBuffers = 3, kVBuffers = 3;
+constexpr uint32_t kPlan = 64;  // tiles whose rows and scales are worked out at a time
 constexpr float kProbLimit = 16384.0f;  // a row's probabilities of a sub-tile may sum to this much
 
 template <int kD>
@@ -45,7 +46,7 @@ struct Shape {
     static constexpr int kVPitch = kD;      // halves, 64-byte chunks swizzled with the key
     static constexpr int kKTile = kBN * kKPitch, kVTile = kBN * kVPitch;
     static constexpr size_t kTileBytes = size_t(kKBuffers * kKTile + kVBuffers * kVTile) * sizeof(uint16_t);
-    static constexpr size_t kLdsBytes = kTileBytes + kKBuffers * 4 * sizeof(float4v) + 16;
+    static constexpr size_t kLdsBytes = kTileBytes + 2 * kPlan * 4 * sizeof(float4v) + 16;
     static constexpr int kSteps = kD / 16;   // MFMAs of the scores of a sub-tile
     static constexpr int kBlocks = kD / 32;  // 32-row head-dim blocks of O^T
     static constexpr int kPhase = kSteps + 2 * kBlocks;
@@ -72,9 +73,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     extern __shared__ __attribute__((aligned(16))) uint16_t s_mem[];
     uint16_t* const s_k0 = s_mem;
     uint16_t* const s_v0 = s_mem + kKBuffers * kKTile;
-    // of run i of the tile in K buffer b: scale of the scores, log2 of the V scale, its inverse, valid
+    // of run i of the workgroup's j-th tile, at (j mod 128) * 4 + i: scale of the scores, log2 of the V scale, its inverse, valid
     float4v* const s_run = reinterpret_cast<float4v*>(reinterpret_cast<unsigned char*>(s_mem) + S::kTileBytes);
-    uint32_t* const s_special = reinterpret_cast<uint32_t*>(s_run + kKBuffers * 4);
+    uint32_t* const s_special = reinterpret_cast<uint32_t*>(s_run + 2 * kPlan * 4);
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = ex_uniform(tid >> 6);
     const uint32_t n = lane & 31, g = lane >> 5;
@@ -170,34 +171,62 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     const uint8_t* const k_base = p.k + int64_t(kvh) * p.head_bytes + (kF8 ? e0 : 2 * e0);
     const uint8_t* const v_base = p.v + int64_t(kvh) * p.head_bytes + (kF8 ? e0 : 2 * e0);
 
-    // The 8 keys of a wave's pieces lie in one run of 16, so the block-table entry, the address of their first row and
-    // their scales are the wave's; a lane adds its row's and column's offset.
+    // The 8 keys of a wave's pieces lie in one run of 16, so the address of their first row is the wave's; a lane
+    // adds its row's and column's offset.  Rows and scales are worked out for 64 tiles at a time, a lane per tile,
+    // and read back lane by lane: per tile that left two scalar reads of what had been lookups, divisions and
+    // conversions in the shadow of too few MFMAs (512 queries at 32768: 559 us before, 538 with it; a window of 4096 at
+    // head size 64: 217 and 204).
     const uint32_t wave_key = 8 * wave;
     const uint32_t lane_off = (ld_r & 7) * uint32_t(p.row_bytes);
     auto key_of = [&](uint32_t it) __attribute__((always_inline)) { return seen.tile(it) * kBN; };  // first key of the it-th tile
-    auto staged = [&](uint32_t it) __attribute__((always_inline)) { return key_of(min(it, n_tiles - 1)); };
-    struct Place {
-        uint32_t blk, in;  // block-table index and row in the block of the wave's first key
+    // lane u: of the wave's keys in tile t_begin + 64 block + u (the last one again behind it)
+    auto plan_key = [&](uint32_t block) __attribute__((always_inline)) {
+        const uint32_t it = min(t_begin + kPlan * block + lane, n_tiles - 1);
+        return min(seen.tile(it) * kBN + wave_key, (seen.end - 1) & ~7u);
     };
-    auto place_of = [&](uint32_t it) __attribute__((always_inline)) -> Place {
-        const uint32_t key = min(staged(it) + wave_key, (seen.end - 1) & ~7u);
-        Place r;
-        if (p.bs_shift >= 0) {
-            r.blk = key >> p.bs_shift;
-            r.in = key & (p.block_size - 1);
+    // step 1: the block-table entry
+    auto plan_entry = [&](uint32_t block) __attribute__((always_inline)) -> int32_t {
+        if constexpr (kRows == kExContiguous) return 0;
+        else return p.tables[plan_key(block) / p.block_size];
+    };
+    // step 2: pool row of the first key, bit 31: the page is one of the pool's; and the scales of its run
+    struct Plan {
+        uint32_t row;
+        float ks, vs;
+    };
+    auto plan_rows = [&](uint32_t block, int32_t entry) __attribute__((always_inline)) -> Plan {
+        Plan r;
+        const uint32_t key = plan_key(block);
+        r.ks = r.vs = 1.0f;
+        if constexpr (kRows == kExContiguous) {
+            r.row = key | 0x80000000u;
         } else {
-            r.blk = key / p.block_size;
-            r.in = key - r.blk * p.block_size;
+            const bool valid = pool_row(entry, key % p.block_size, p.block_size, p.num_blocks, &r.row);
+            if constexpr (kF8) {
+                const uint64_t at = uint64_t(valid ? uint32_t(entry) : 0u) * p.num_kv_heads + kvh;
+                r.ks = p.k_scale[at];
+                r.vs = p.v_scale[at];
+            }
+            r.row |= valid ? 0x80000000u : 0u;
         }
         return r;
     };
-    auto lookup = [&](uint32_t it) __attribute__((always_inline)) -> int32_t {  // the entry, one value for the wave
-        if constexpr (kRows == kExContiguous) return 0;
-        else return p.tables[place_of(it).blk];
+    // step 3: what the softmax takes from the scales, for every wave.  A run that nobody sees may have anything for
+    // scales; a masked score, minus infinity, must come through the factor and the shift as what it is: a positive
+    // factor, a finite shift.
+    auto plan_runs = [&](const Plan& r, uint32_t half) __attribute__((always_inline)) {
+        if (kRows == kExContiguous || (wave & 1)) return;  // (waves 2 i and 2 i + 1 have the same run)
+        const bool valid = r.row >> 31;
+        const float vs = kF8 && valid ? fminf(fmaxf(r.vs, 0x1p-100f), 0x1p+126f) : 1.0f;
+        float4v info;
+        info.x = kF8 && valid ? fmaxf(fmaxf(r.ks, 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
+        info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
+        info.z = 1.0f / vs;
+        info.w = valid ? 1.0f : 0.0f;
+        s_run[(half * kPlan + lane) * 4 + (wave >> 1)] = info;
     };
     struct Piece {
         uint32_t k[kRegs], v[kRegs];
-        float ks, vs;  // of the run of its K
     };
     auto fetch = [&](uint32_t (&dst)[kRegs], const uint8_t* src) __attribute__((always_inline)) {
         if constexpr (kRegs == 2) {
@@ -213,37 +242,18 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             }
         }
     };
-    // Row of the wave's first key of tile `it` (its validity in `valid`), from its table entry.
-    struct RowAt {
-        uint32_t row, valid;
-    };
-    auto row_at = [&](uint32_t it, int32_t entry) __attribute__((always_inline)) -> RowAt {
-        RowAt r;
-        r.valid = 1;
-        if constexpr (kRows == kExContiguous) {
-            r.row = staged(it);
-        } else {
-            r.valid = pool_row(int32_t(ex_uniform(uint32_t(entry))), place_of(it).in, p.block_size, p.num_blocks, &r.row) ? 1u : 0u;
-        }
-        return r;
-    };
-    auto piece_at = [&](const uint8_t* base, const RowAt& r) __attribute__((always_inline)) -> const uint8_t* {
+    // `at`: a tile's planned row, one value for the wave
+    auto piece_at = [&](const uint8_t* base, uint32_t at) __attribute__((always_inline)) -> const uint8_t* {
+        const uint32_t row = at & 0x7FFFFFFFu;
         if constexpr (kRows == kExContiguous) {
             // (rows behind the last key may lie behind the cache's end: the last one instead)
-            return base + uint64_t(min(r.row + ld_r, len - 1)) * uint64_t(p.row_bytes);
+            return base + uint64_t(min(row + (ld_r & 7), len - 1)) * uint64_t(p.row_bytes);
         } else {
-            return base + uint64_t(r.row) * uint64_t(p.row_bytes) + lane_off;
+            return base + uint64_t(row) * uint64_t(p.row_bytes) + lane_off;
         }
     };
-    auto load_k = [&](const RowAt& r, int32_t entry, Piece& piece) __attribute__((always_inline)) {
-        if constexpr (kF8) {
-            const uint64_t sc = uint64_t(r.valid ? ex_uniform(uint32_t(entry)) : 0u) * p.num_kv_heads + kvh;
-            piece.ks = p.k_scale[sc];
-            piece.vs = p.v_scale[sc];
-        }
-        fetch(piece.k, piece_at(k_base, r));
-    };
-    auto load_v = [&](const RowAt& r, Piece& piece) __attribute__((always_inline)) { fetch(piece.v, piece_at(v_base, r)); };
+    auto load_k = [&](uint32_t at, Piece& piece) __attribute__((always_inline)) { fetch(piece.k, piece_at(k_base, at)); };
+    auto load_v = [&](uint32_t at, Piece& piece) __attribute__((always_inline)) { fetch(piece.v, piece_at(v_base, at)); };
     auto halves_of = [&](const uint32_t (&src)[kRegs], int half) __attribute__((always_inline)) -> uint4v {
         if constexpr (kF8) {
             return __builtin_bit_cast(uint4v, f8x8_to_half8(src[2 * half], src[2 * half + 1]));
@@ -251,21 +261,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             return uint4v{src[4 * half], src[4 * half + 1], src[4 * half + 2], src[4 * half + 3]};
         }
     };
-    auto store_k = [&](uint32_t buf, uint32_t valid, const Piece& piece) __attribute__((always_inline)) {
+    auto store_k = [&](uint32_t buf, const Piece& piece) __attribute__((always_inline)) {
         uint16_t* s = s_k0 + buf * kKTile;
         *reinterpret_cast<uint4v*>(s + k_st0) = halves_of(piece.k, 0);
         if constexpr (kTwo) *reinterpret_cast<uint4v*>(s + k_st1) = halves_of(piece.k, 1);
-        if (kRows != kExContiguous && (tid & 127) == 0) {  // one thread per run
-            // (a run that nobody sees may have anything for scales; a masked score, minus infinity, must come
-            // through the factor and the shift as what it is: a positive factor, a finite shift)
-            const float vs = kF8 && valid ? fminf(fmaxf(piece.vs, 0x1p-100f), 0x1p+126f) : 1.0f;
-            float4v info;
-            info.x = kF8 && valid ? fmaxf(fmaxf(piece.ks, 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
-            info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
-            info.z = 1.0f / vs;
-            info.w = valid ? 1.0f : 0.0f;
-            s_run[buf * 4 + (tid >> 7)] = info;
-        }
     };
     // Whether some row of the workgroup does not see some key of the tile that begins at key0.
     auto partial = [&](uint32_t key0) __attribute__((always_inline)) {
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         uint16_t* s = s_v0 + buf * kVTile;
         uint4v x0 = halves_of(piece.v, 0), x1 = {0, 0, 0, 0};
         if constexpr (kTwo) x1 = halves_of(piece.v, 1);
-        const uint32_t key0 = staged(it);
+        const uint32_t key0 = key_of(min(it, n_tiles - 1));
         if (partial(key0) || (kRows != kExContiguous && !valid)) {
             const uint32_t key = key0 + ld_r;
             bool special = drop_specials(x0);
@@ -314,13 +313,14 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         bool valid;  // both
         uint32_t bits;
     };
-    auto runs_of = [&](uint32_t kbuf, int sub) __attribute__((always_inline)) -> Runs {
+    auto runs_of = [&](uint32_t it, int sub) __attribute__((always_inline)) -> Runs {
         Runs x;
         x.bits = 3;
         if constexpr (kRows == kExContiguous) {
             x.r[0] = x.r[1] = Run{p.scale_log2, 0.0f, 1.0f};
         } else {
-            const float4v a = s_run[kbuf * 4 + 2 * sub], b = s_run[kbuf * 4 + 2 * sub + 1];
+            const uint32_t at = (it - t_begin) % (2 * kPlan) * 4 + 2 * sub;
+            const float4v a = s_run[at], b = s_run[at + 1];
             x.bits = ex_uniform((a.w != 0.0f ? 1u : 0u) | (b.w != 0.0f ? 2u : 0u));
             if constexpr (kF8) {
                 x.r[0] = Run{a.x, a.y, a.z};
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     };
     // One phase of the pipeline: scores of sub-tile j + 1 (key0_q, buffer kbuf), softmax of j (s_in, runs_in), second
     // product of j - 1.  `side(step)` is the caller's work in the shadow of the MFMAs.
-    auto fused_phase = [&](uint32_t key0_q, uint32_t kbuf, int sub_q, float16v& s_out, const float16v& s_in, const Runs& runs_in,
+    auto fused_phase = [&](uint32_t it_q, uint32_t key0_q, uint32_t kbuf, int sub_q, float16v& s_out, const float16v& s_in, const Runs& runs_in,
                            Probs& p_out, uint32_t vbuf, int sub_v, const Probs& p_prev, auto&& side) __attribute__((always_inline)) {
         const uint16_t* krow = s_k0 + kbuf * kKTile + (32 * sub_q + n) * kKPitch + 8 * g;
         const uint16_t* sv = s_v0 + vbuf * kVTile + 32 * sub_v * kVPitch;
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         }
 #pragma unroll
         for (int i = 0; i < kRing - 1; i++) ring[i] = v_operand(i);
-        apply_mask(key0_q, kRows == kExContiguous ? 3u : runs_of(kbuf, sub_q).bits, c);  // rare
+        apply_mask(key0_q, kRows == kExContiguous ? 3u : runs_of(it_q, sub_q).bits, c);  // rare
 #pragma unroll
         for (int i = 0; i < 2 * kBlocks; i++) {
             if (i + kRing - 1 < 2 * kBlocks) ring[(i + kRing - 1) % kRing] = v_operand(i + kRing - 1);
@@ -511,30 +511,30 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         my_end += (my_end - t_begin) & 1;
 
         // ---- prologue: in LDS K of the first two tiles and V of the first, in flight K of the third and fourth and V of
-        // the second and third, lookups two tiles further
+        // the second and third, and the rows of the first 64
         Piece a, b;
-        const int32_t e0_ = lookup(t_begin), e1_ = lookup(t_begin + 1), e2_ = lookup(t_begin + 2), e3_ = lookup(t_begin + 3);
-        const RowAt o0 = row_at(t_begin, e0_), o1 = row_at(t_begin + 1, e1_), o2 = row_at(t_begin + 2, e2_), o3 = row_at(t_begin + 3, e3_);
-        load_k(o0, e0_, a);
+        Plan cur = plan_rows(0, plan_entry(0));
+        int32_t next_entry = 0;
+        Plan next = cur;
+        auto row_of = [&](uint32_t j) __attribute__((always_inline)) { return uint32_t(__builtin_amdgcn_readlane(int(cur.row), int(j % kPlan))); };
+        const uint32_t o0 = row_of(0), o1 = row_of(1), o2 = row_of(2), o3 = row_of(3);
+        load_k(o0, a);
         load_v(o0, a);
-        load_k(o1, e1_, b);
-        store_k(0, o0.valid, a);
-        store_v(0, t_begin, o0.valid, a);
-        store_k(1, o1.valid, b);
+        load_k(o1, b);
+        plan_runs(cur, 0);
+        plan_runs(cur, 1);  // (tiles behind the last, which are masked, find valid numbers)
+        store_k(0, a);
+        store_v(0, t_begin, o0 >> 31, a);
+        store_k(1, b);
         __builtin_amdgcn_sched_barrier(0);
-        load_k(o2, e2_, a);
+        load_k(o2, a);
         load_v(o1, a);
         __builtin_amdgcn_sched_barrier(0);
-        int32_t look_a = lookup(t_begin + 4);
-        __builtin_amdgcn_sched_barrier(0);
-        load_k(o3, e3_, b);
+        load_k(o3, b);
         load_v(o2, b);
         __builtin_amdgcn_sched_barrier(0);
-        int32_t look_b = lookup(t_begin + 5);
-        __builtin_amdgcn_sched_barrier(0);
-        RowAt at_v = o3;  // of the tile whose V is loaded next
-        // validity of the tiles in flight: K of it + 2 and it + 3, V of it + 1 and it + 2 (bit 0 the nearer)
-        uint32_t k_valid = o2.valid | (o3.valid << 1), v_valid = o1.valid | (o2.valid << 1);
+        uint32_t at_v = o3;                   // of the tile whose V is loaded next
+        uint32_t at_v1 = o1, at_v2 = o2;      // of those whose V is in flight: stored next, and the one after
         __syncthreads();
 
         float16v s0, s1;
@@ -546,23 +546,32 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         }
         if (my_end > t_begin) {
             scores(0, 0, s0);
-            apply_mask(key_of(t_begin), runs_of(0, 0).bits, s0);
+            apply_mask(key_of(t_begin), runs_of(t_begin, 0).bits, s0);
         }
         uint32_t kb_cur = 0, kb_next = 1, kb_store = 2;
         // (the first iteration's second product, of nothing, reads the first tile's V: whatever it holds, every row sees it)
         uint32_t vb_prev = 0, vb_cur = 0, vb_store = 1;
-        auto staging = [&](uint32_t it, Piece& piece, int32_t& look, int part) __attribute__((always_inline)) {
-            if (part == 0) store_k(kb_store, k_valid & 1, piece);           // K of tile it + 2
-            if (part == 2) store_v(vb_store, it + 1, v_valid & 1, piece);   // V of tile it + 1
-            if (part == 4) {
-                const RowAt at_k = row_at(it + 4, look);  // K of it + 4, V of it + 3
-                load_k(at_k, look, piece);
+        auto staging = [&](uint32_t it, Piece& piece, int part) __attribute__((always_inline)) {
+            if (part == 0) store_k(kb_store, piece);                      // K of tile it + 2
+            if (part == 2) store_v(vb_store, it + 1, at_v1 >> 31, piece); // V of tile it + 1
+            if (part == 4) {  // K of it + 4, V of it + 3
+                const uint32_t j = it + 4 - t_begin;
+                if (j % kPlan == 0) cur = next;
+                const uint32_t at_k = row_of(j);
+                load_k(at_k, piece);
                 load_v(at_v, piece);
-                k_valid = (k_valid >> 1) | (at_k.valid << 1);
-                v_valid = (v_valid >> 1) | (at_v.valid << 1);
+                at_v1 = at_v2;
+                at_v2 = at_v;
                 at_v = at_k;
             }
-            if (part == 5) look = lookup(it + 6);
+            if (part == 5) {  // the next 64 tiles, in three steps a few tiles apart
+                const uint32_t j = it + 4 - t_begin, block = j / kPlan + 1;
+                if (t_begin + block * kPlan < n_tiles) {
+                    if (j % kPlan == 32) next_entry = plan_entry(block);
+                    else if (j % kPlan == 40) next = plan_rows(block, next_entry);
+                    else if (j % kPlan == 48) plan_runs(next, block & 1);
+                }
+            }
         };
         auto rotate_buffers = [&]() __attribute__((always_inline)) {
             __syncthreads();
@@ -574,28 +583,37 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             vb_cur = vb_store;
             vb_store = 3 - vb_prev - vb_cur;
         };
-        auto iteration = [&](uint32_t it, Piece& piece, int32_t& look) __attribute__((always_inline)) {
+        // At head size 64 a phase has too few MFMAs to cover all of the staging: it is spread over both (196 us against
+        // 204 for 4096 queries with a window of 4096; at 128 the second phase covers nothing more: 550 against 538 for 512 at 32768).
+        constexpr bool kSpread = kD == 64;
+        auto iteration = [&](uint32_t it, Piece& piece) __attribute__((always_inline)) {
             const uint32_t key_cur = key_of(it), key_nxt = key_of(it + 1);
-            const Runs ra = runs_of(kb_cur, 0);
-            fused_phase(key_cur + 32, kb_cur, 1, s1, s0, ra, p_new, vb_prev, 1, p_old, [&](int step) { staging(it, piece, look, step - (kPhase - 8)); });
-            const Runs rb = runs_of(kb_cur, 1);
-            fused_phase(key_nxt, kb_next, 0, s0, s1, rb, p_old, vb_cur, 0, p_new, [](int) {});
+            const Runs ra = runs_of(it, 0);
+            fused_phase(it, key_cur + 32, kb_cur, 1, s1, s0, ra, p_new, vb_prev, 1, p_old, [&](int step) {
+                const int part = step - (kPhase - 8);
+                if (!kSpread || part == 0) staging(it, piece, part);
+            });
+            const Runs rb = runs_of(it, 1);
+            fused_phase(it + 1, key_nxt, kb_next, 0, s0, s1, rb, p_old, vb_cur, 0, p_new, [&](int step) {
+                const int part = step - (kPhase - 8) + 2;
+                if (kSpread && part >= 2) staging(it, piece, part);
+            });
             rotate_buffers();
         };
-        auto stage_only = [&](uint32_t it, Piece& piece, int32_t& look) __attribute__((always_inline)) {
+        auto stage_only = [&](uint32_t it, Piece& piece) __attribute__((always_inline)) {
 #pragma unroll
-            for (int part = 0; part < 6; part++) staging(it, piece, look, part);
+            for (int part = 0; part < 6; part++) staging(it, piece, part);
             rotate_buffers();
         };
         uint32_t it = t_begin;
         for (; it < my_end; it += 2) {
-            iteration(it, a, look_a);
-            iteration(it + 1, b, look_b);
+            iteration(it, a);
+            iteration(it + 1, b);
         }
         if (my_end > t_begin) accumulate(vb_prev, 1, p_old);
         for (; it < n_tiles; it += 2) {
-            stage_only(it, a, look_a);
-            stage_only(it + 1, b, look_b);
+            stage_only(it, a);
+            stage_only(it + 1, b);
         }
     }
 
