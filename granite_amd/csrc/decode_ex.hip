@@ -11,6 +11,7 @@ namespace {
 constexpr uint32_t kRowWaves = 8;
 constexpr uint32_t kDirectTokens = 768;
 constexpr uint32_t kStreamRows = 320, kStreamRowsHalf = 160;  // float, half results
+constexpr uint32_t kFewRows = 32, kFewRowsTokens = 6144;
 
 // One workgroup per (run of 16 query rows, KV head, sequence, key split).  A row is a (query, head of
 // the KV head's group) pair, row r = query * group + head, so a decode step's group, a few draft tokens and a
@@ -344,15 +345,18 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     p.causal = a.mask_mode == GRANITE_HIP_MASK_CAUSAL;
     p.start_pos = a.start_pos;
     p.scale_log2 = a.scale * kExLog2e;
-    // Few rows of 8-bit pools: the persistent kernel of the decode step, 16 rows in the place of a head's group
+    // Few rows of 8-bit pools: the persistent kernel of the decode step, 16 rows in the place of a head's group.  A draft's
+    // worth of them on few keys is quicker on the row kernel (8 queries of 32 heads over 8 KV heads, half results: 200 keys
+    // 8.7 us against 11.7, 4096 keys 16.8 against 20.0; 32768 keys 36.5 against 34.0).
     const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3;
-    if (f8 && rows == kExPaged16 && uint64_t(a.seq_q) * p.group <= (p.out_f32 ? kStreamRows : kStreamRowsHalf)) {
-        const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
+    const uint64_t n_rows = uint64_t(a.seq_q) * p.group;
+    const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
+    if (f8 && rows == kExPaged16 && n_rows <= (p.out_f32 ? kStreamRows : kStreamRowsHalf) && (n_rows > kFewRows || seen > kFewRowsTokens)) {
         const uint32_t tiles = uint32_t((seen + 31) / 32);
-        p.q_groups = uint32_t((uint64_t(a.seq_q) * p.group + 15) / 16);
+        p.q_groups = uint32_t((n_rows + 15) / 16);
         if (kv_stream_supports(p, tiles)) return launch_kv_stream(p, D, a.q_dtype == GRANITE_HIP_F32, f8, rows, tiles, scratch);
     }
-    if (rows != kExPagedAny && uint64_t(a.seq_q) * p.group > 32)
+    if (rows != kExPagedAny && n_rows > kFewRows)
         return launch_kv_tiles(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
     return launch_rows(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
 }

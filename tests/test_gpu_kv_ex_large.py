@@ -7,7 +7,7 @@ import pytest
 import kv8
 from granite_amd import F16, F32, F8E4M3, MASK_CAUSAL
 from gpu_util import dev, say
-from test_gpu_kv_ex import check, v_top
+from test_gpu_kv_ex import NAN8, Cache, check, run_prefill, v_top
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +111,20 @@ def test_prefill_many_tiles_in_one_go(gpu, kv, window, sinks, q_dtype, out_dtype
         vis = kv8.visible(start + np.asarray(some), start + n, window, sinks)
         o, l, ds = kv8.attend(q[some, heads], k, v, vis, d ** -0.5)
         check(got[some, heads], got_lse[some, heads], o, l, ds, v_top(v, vis), int(vis.sum(1).max()), out_dtype == F16, f"head {kvh}")
+
+
+@pytest.mark.parametrize("n,start,bs,hq,hkv,d", [(1, 7000, 16, 8, 2, 128), (2, 6600, 32, 4, 4, 64), (3, 8100, 48, 16, 2, 128), (4, 6143, 16, 7, 1, 64)])
+@pytest.mark.parametrize("q_dtype,out_dtype", [(F16, F16), (F32, F32)])
+def test_prefill_few_rows_many_keys(gpu, n, start, bs, hq, hkv, d, q_dtype, out_dtype):
+    """A draft's worth of queries behind a long context, with released pages and NaNs that not every query sees."""
+    say(f"prefill few rows n={n} start={start} bs={bs}")
+    cache = Cache(np.random.default_rng(n), [start + n], bs, hkv, d, F8E4M3)
+    for j in range(20, 30):
+        cache.table[0, j] = (-1, cache.num_blocks, 2147483647)[j % 3]
+    at = lambda t: cache.table[0, t // bs] * bs + t % bs  # noqa: E731
+    cache.v[at(start + n // 2), 0, 3] = NAN8          # the later queries'
+    cache.v[at(start - 6200), 0, 4] = NAN8            # behind the window, of those without one
+    cache.upload()
+    run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype)
+    run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype, 6190, 5)
+    run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype, 6200 + n // 2, 0)   # the first queries'
