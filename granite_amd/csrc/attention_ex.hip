@@ -13,8 +13,9 @@
 // * Codes become halves once per workgroup, on the way from registers to LDS (v_cvt_scalef32_pk_f16_fp8,
 //   two codes an instruction): a half holds every e4m3 value, so the products are those of the codes themselves.  Converting
 //   operands as they are read would put four conversions beside every MFMA of every wave.
-// * Scales never touch an element of K or V.  A run of 16 keys lies in one block (block sizes are multiples of
-//   16 here), so a sub-tile has two scales of K and two of V.  K's goes into the factor that takes a score to the
+// * Scales never touch an element of K or V.  Where block sizes are multiples of 16 a run of 16 keys lies in one block, so
+//   a sub-tile has two scales of K and two of V; where they are other multiples of 4 (kExPaged4) a run of 4 does, which
+//   are the rows 8 a + 4 g .. + 3 that lane (n, g) has of its column: four scales a lane instead of two.  K's goes into the factor that takes a score to the
 //   log2 domain.  V's enters the exponent: with x = score + log2(v scale) the probabilities p' = exp2(x - ref)
 //   carry it, the second product takes the codes, and the sum l takes each run's p' times 1 / (v scale).  The
 //   reference follows x, so a large or small V scale never pushes p' out of the range of a half.  Cost per sub-tile:
@@ -40,13 +41,15 @@ constexpr int kKBuffers = 3, kVBuffers = 3;
 constexpr uint32_t kPlan = 64;  // tiles whose rows and scales are worked out at a time
 constexpr float kProbLimit = 16384.0f;  // a row's probabilities of a sub-tile may sum to this much
 
-template <int kD>
+template <int kD, int kRows>
 struct Shape {
+    static constexpr uint32_t kRun = kRows == kExPaged4 ? 4 : 16;  // keys that are sure to lie in one block
+    static constexpr uint32_t kTileRuns = kBN / kRun;
     static constexpr int kKPitch = kD + 8;  // halves
     static constexpr int kVPitch = kD;      // halves, 64-byte chunks swizzled with the key
     static constexpr int kKTile = kBN * kKPitch, kVTile = kBN * kVPitch;
     static constexpr size_t kTileBytes = size_t(kKBuffers * kKTile + kVBuffers * kVTile) * sizeof(uint16_t);
-    static constexpr size_t kLdsBytes = kTileBytes + 2 * kPlan * 4 * sizeof(float4v) + 16;
+    static constexpr size_t kLdsBytes = kTileBytes + 2 * kPlan * kTileRuns * sizeof(float4v) + 16;
     static constexpr int kSteps = kD / 16;   // MFMAs of the scores of a sub-tile
     static constexpr int kBlocks = kD / 32;  // 32-row head-dim blocks of O^T
     static constexpr int kPhase = kSteps + 2 * kBlocks;
@@ -67,15 +70,18 @@ __device__ __forceinline__ bool drop_specials(uint4v& x) {
 
 template <bool kQF32, bool kPrecise, bool kF8, int kRows, int kD>
 __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
-    using S = Shape<kD>;
+    using S = Shape<kD, kRows>;
+    constexpr bool kFine = kRows == kExPaged4;
+    constexpr uint32_t kTileRuns = S::kTileRuns;
+    constexpr int kLaneRuns = kFine ? 4 : 2, kRunShift = kFine ? 2 : 3;  // of the 16 scores a lane has of a sub-tile
     constexpr int kKPitch = S::kKPitch, kVPitch = S::kVPitch, kKTile = S::kKTile, kVTile = S::kVTile, kSteps = S::kSteps,
                   kBlocks = S::kBlocks, kPhase = S::kPhase;
     extern __shared__ __attribute__((aligned(16))) uint16_t s_mem[];
     uint16_t* const s_k0 = s_mem;
     uint16_t* const s_v0 = s_mem + kKBuffers * kKTile;
-    // of run i of the workgroup's j-th tile, at (j mod 128) * 4 + i: scale of the scores, log2 of the V scale, its inverse, valid
+    // of run i of the workgroup's j-th tile, at (j mod 128) * kTileRuns + i: scale of the scores, log2 of the V scale, its inverse, valid
     float4v* const s_run = reinterpret_cast<float4v*>(reinterpret_cast<unsigned char*>(s_mem) + S::kTileBytes);
-    uint32_t* const s_special = reinterpret_cast<uint32_t*>(s_run + 2 * kPlan * 4);
+    uint32_t* const s_special = reinterpret_cast<uint32_t*>(s_run + 2 * kPlan * kTileRuns);
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = ex_uniform(tid >> 6);
     const uint32_t n = lane & 31, g = lane >> 5;
@@ -171,43 +177,53 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     const uint8_t* const k_base = p.k + int64_t(kvh) * p.head_bytes + (kF8 ? e0 : 2 * e0);
     const uint8_t* const v_base = p.v + int64_t(kvh) * p.head_bytes + (kF8 ? e0 : 2 * e0);
 
-    // The 8 keys of a wave's pieces lie in one run of 16, so the address of their first row is the wave's; a lane
-    // adds its row's and column's offset.  Rows and scales are worked out for 64 tiles at a time, a lane per tile,
+    // The 8 keys of a wave's pieces lie in one run of 16 (in two of 4), so the address of a run's first row is the wave's; a
+    // lane adds its row's and column's offset.  Rows and scales are worked out for 64 tiles at a time, a lane per tile,
     // and read back lane by lane: per tile that left two scalar reads of what had been lookups, divisions and
     // conversions in the shadow of too few MFMAs (512 queries at 32768: 559 us before, 538 with it; a window of 4096 at
     // head size 64: 217 and 204).
+    constexpr int kPieceRuns = kFine ? 2 : 1;
     const uint32_t wave_key = 8 * wave;
-    const uint32_t lane_off = (ld_r & 7) * uint32_t(p.row_bytes);
+    const uint32_t lane_off = (ld_r & (kFine ? 3 : 7)) * uint32_t(p.row_bytes);
     auto key_of = [&](uint32_t it) __attribute__((always_inline)) { return seen.tile(it) * kBN; };  // first key of the it-th tile
-    // lane u: of the wave's keys in tile t_begin + 64 block + u (the last one again behind it)
-    auto plan_key = [&](uint32_t block) __attribute__((always_inline)) {
+    // lane u: first key of run f of the wave's keys in tile t_begin + 64 block + u (the last one again behind it)
+    auto plan_key = [&](uint32_t block, int f) __attribute__((always_inline)) {
         const uint32_t it = min(t_begin + kPlan * block + lane, n_tiles - 1);
-        return min(seen.tile(it) * kBN + wave_key, (seen.end - 1) & ~7u);
+        return min(seen.tile(it) * kBN + wave_key + 4 * f, (seen.end - 1) & (kFine ? ~3u : ~7u));
     };
-    // step 1: the block-table entry
-    auto plan_entry = [&](uint32_t block) __attribute__((always_inline)) -> int32_t {
-        if constexpr (kRows == kExContiguous) return 0;
-        else return p.tables[plan_key(block) / p.block_size];
+    // step 1: the block-table entries
+    struct Entries {
+        int32_t e[kPieceRuns];
+    };
+    auto plan_entries = [&](uint32_t block) __attribute__((always_inline)) -> Entries {
+        Entries r;
+#pragma unroll
+        for (int f = 0; f < kPieceRuns; f++) r.e[f] = kRows == kExContiguous ? 0 : p.tables[plan_key(block, f) / p.block_size];
+        return r;
     };
     // step 2: pool row of the first key, bit 31: the page is one of the pool's; and the scales of its run
     struct Plan {
-        uint32_t row;
-        float ks, vs;
+        uint32_t row[kPieceRuns];
+        float ks[kPieceRuns], vs[kPieceRuns];
     };
-    auto plan_rows = [&](uint32_t block, int32_t entry) __attribute__((always_inline)) -> Plan {
+    auto plan_rows = [&](uint32_t block, const Entries& entries) __attribute__((always_inline)) -> Plan {
         Plan r;
-        const uint32_t key = plan_key(block);
-        r.ks = r.vs = 1.0f;
-        if constexpr (kRows == kExContiguous) {
-            r.row = key | 0x80000000u;
-        } else {
-            const bool valid = pool_row(entry, key % p.block_size, p.block_size, p.num_blocks, &r.row);
-            if constexpr (kF8) {
-                const uint64_t at = uint64_t(valid ? uint32_t(entry) : 0u) * p.num_kv_heads + kvh;
-                r.ks = p.k_scale[at];
-                r.vs = p.v_scale[at];
+#pragma unroll
+        for (int f = 0; f < kPieceRuns; f++) {
+            const uint32_t key = plan_key(block, f);
+            r.ks[f] = r.vs[f] = 1.0f;
+            if constexpr (kRows == kExContiguous) {
+                r.row[f] = key | 0x80000000u;
+            } else {
+                const int32_t entry = entries.e[f];
+                const bool valid = pool_row(entry, key % p.block_size, p.block_size, p.num_blocks, &r.row[f]);
+                if constexpr (kF8) {
+                    const uint64_t at = uint64_t(valid ? uint32_t(entry) : 0u) * p.num_kv_heads + kvh;
+                    r.ks[f] = p.k_scale[at];
+                    r.vs[f] = p.v_scale[at];
+                }
+                r.row[f] |= valid ? 0x80000000u : 0u;
             }
-            r.row |= valid ? 0x80000000u : 0u;
         }
         return r;
     };
@@ -215,15 +231,22 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     // scales; a masked score, minus infinity, must come through the factor and the shift as what it is: a positive
     // factor, a finite shift.
     auto plan_runs = [&](const Plan& r, uint32_t half) __attribute__((always_inline)) {
-        if (kRows == kExContiguous || (wave & 1)) return;  // (waves 2 i and 2 i + 1 have the same run)
-        const bool valid = r.row >> 31;
-        const float vs = kF8 && valid ? fminf(fmaxf(r.vs, 0x1p-100f), 0x1p+126f) : 1.0f;
-        float4v info;
-        info.x = kF8 && valid ? fmaxf(fmaxf(r.ks, 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
-        info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
-        info.z = 1.0f / vs;
-        info.w = valid ? 1.0f : 0.0f;
-        s_run[(half * kPlan + lane) * 4 + (wave >> 1)] = info;
+        if (kRows == kExContiguous || (!kFine && (wave & 1))) return;  // (waves 2 i and 2 i + 1 have the same run of 16)
+#pragma unroll
+        for (int f = 0; f < kPieceRuns; f++) {
+            const bool valid = r.row[f] >> 31;
+            const float vs = kF8 && valid ? fminf(fmaxf(r.vs[f], 0x1p-100f), 0x1p+126f) : 1.0f;
+            float4v info;
+            info.x = kF8 && valid ? fmaxf(fmaxf(r.ks[f], 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
+            info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
+            info.z = 1.0f / vs;
+            info.w = valid ? 1.0f : 0.0f;
+            s_run[(half * kPlan + lane) * kTileRuns + (kFine ? 2 * wave + f : wave >> 1)] = info;
+        }
+    };
+    // a tile's planned rows: one value for the wave, or one for its first four keys and one for the others
+    struct At {
+        uint32_t row[kPieceRuns];
     };
     struct Piece {
         uint32_t k[kRegs], v[kRegs];
@@ -242,9 +265,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             }
         }
     };
-    // `at`: a tile's planned row, one value for the wave
-    auto piece_at = [&](const uint8_t* base, uint32_t at) __attribute__((always_inline)) -> const uint8_t* {
-        const uint32_t row = at & 0x7FFFFFFFu;
+    auto of_lane = [&](const At& at) __attribute__((always_inline)) -> uint32_t {
+        if constexpr (kFine) return ld_r & 4 ? at.row[1] : at.row[0];
+        else return at.row[0];
+    };
+    auto piece_at = [&](const uint8_t* base, const At& at) __attribute__((always_inline)) -> const uint8_t* {
+        const uint32_t row = of_lane(at) & 0x7FFFFFFFu;
         if constexpr (kRows == kExContiguous) {
             // (rows behind the last key may lie behind the cache's end: the last one instead)
             return base + uint64_t(min(row + (ld_r & 7), len - 1)) * uint64_t(p.row_bytes);
@@ -252,8 +278,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             return base + uint64_t(row) * uint64_t(p.row_bytes) + lane_off;
         }
     };
-    auto load_k = [&](uint32_t at, Piece& piece) __attribute__((always_inline)) { fetch(piece.k, piece_at(k_base, at)); };
-    auto load_v = [&](uint32_t at, Piece& piece) __attribute__((always_inline)) { fetch(piece.v, piece_at(v_base, at)); };
+    auto load_k = [&](const At& at, Piece& piece) __attribute__((always_inline)) { fetch(piece.k, piece_at(k_base, at)); };
+    auto load_v = [&](const At& at, Piece& piece) __attribute__((always_inline)) { fetch(piece.v, piece_at(v_base, at)); };
     auto halves_of = [&](const uint32_t (&src)[kRegs], int half) __attribute__((always_inline)) -> uint4v {
         if constexpr (kF8) {
             return __builtin_bit_cast(uint4v, f8x8_to_half8(src[2 * half], src[2 * half + 1]));
@@ -270,7 +296,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     auto partial = [&](uint32_t key0) __attribute__((always_inline)) {
         return key0 + kBN > all_hi || (key0 < all_lo && key0 + kBN > p.sinks);
     };
-    auto store_v = [&](uint32_t buf, uint32_t it, uint32_t valid, const Piece& piece) __attribute__((always_inline)) {
+    auto store_v = [&](uint32_t buf, uint32_t it, const At& at, const Piece& piece) __attribute__((always_inline)) {
+        const uint32_t valid = of_lane(at) >> 31;
         uint16_t* s = s_v0 + buf * kVTile;
         uint4v x0 = halves_of(piece.v, 0), x1 = {0, 0, 0, 0};
         if constexpr (kTwo) x1 = halves_of(piece.v, 1);
@@ -309,40 +336,41 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         float scale, lvs, inv;
     };
     struct Runs {
-        Run r[2];
-        bool valid;  // both
-        uint32_t bits;
+        Run r[kLaneRuns];
+        uint32_t bits;  // of those whose page is one of the pool's
     };
+    constexpr uint32_t kAllRuns = (1u << kLaneRuns) - 1;
     auto runs_of = [&](uint32_t it, int sub) __attribute__((always_inline)) -> Runs {
         Runs x;
-        x.bits = 3;
+        x.bits = kAllRuns;
         if constexpr (kRows == kExContiguous) {
             x.r[0] = x.r[1] = Run{p.scale_log2, 0.0f, 1.0f};
         } else {
-            const uint32_t at = (it - t_begin) % (2 * kPlan) * 4 + 2 * sub;
-            const float4v a = s_run[at], b = s_run[at + 1];
-            x.bits = ex_uniform((a.w != 0.0f ? 1u : 0u) | (b.w != 0.0f ? 2u : 0u));
-            if constexpr (kF8) {
-                x.r[0] = Run{a.x, a.y, a.z};
-                x.r[1] = Run{b.x, b.y, b.z};
-            } else {
-                x.r[0] = x.r[1] = Run{p.scale_log2, 0.0f, 1.0f};
+            const uint32_t at = (it - t_begin) % (2 * kPlan) * kTileRuns + (kTileRuns / 2) * sub + (kFine ? g : 0);
+            x.bits = 0;
+#pragma unroll
+            for (int a = 0; a < kLaneRuns; a++) {
+                const float4v r = s_run[at + (kFine ? 2 * a : a)];
+                x.bits |= r.w != 0.0f ? 1u << a : 0u;
+                x.r[a] = kF8 ? Run{r.x, r.y, r.z} : Run{p.scale_log2, 0.0f, 1.0f};
             }
+            if constexpr (!kFine) x.bits = ex_uniform(x.bits);
         }
-        x.valid = x.bits == 3;
         return x;
     };
     // keys of the sub-tile at key0 that the lane's row does not see become minus infinity
     auto apply_mask = [&](uint32_t key0, uint32_t bits, float16v& s) __attribute__((always_inline)) {
-        if (key0 + 32 <= every_hi && (key0 >= every_lo || key0 + 32 <= p.sinks) && bits == 3) return;
+        if (key0 + 32 <= every_hi && (key0 >= every_lo || key0 + 32 <= p.sinks) && (kFine ? __all(bits == kAllRuns) : bits == kAllRuns)) return;
         // what depends on the lane goes into three numbers, the rest is a constant per element; no short-circuit logic,
         // so that it stays compares and selects
         const int32_t base = int32_t(key0 + 4 * g), lo = int32_t(row_lo) - base, sink = int32_t(p.sinks) - base;
-        const int32_t hi[2] = {bits & 1u ? int32_t(row_hi) - base : -1, bits & 2u ? int32_t(row_hi) - base : -1};
+        int32_t hi[kLaneRuns];
+#pragma unroll
+        for (int a = 0; a < kLaneRuns; a++) hi[a] = (bits >> a) & 1u ? int32_t(row_hi) - base : -1;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             const int32_t in = 8 * (r >> 2) + (r & 3);
-            const bool vis = bool(int(in < hi[r >> 3]) & (int(in >= lo) | int(in < sink)));
+            const bool vis = bool(int(in < hi[r >> kRunShift]) & (int(in >= lo) | int(in < sink)));
             s[r] = vis ? s[r] : -INFINITY;
         }
     };
@@ -366,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     auto rebase = [&](const float16v& s, const Runs& runs) __attribute__((always_inline)) {
         float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 16; r++) top = fmaxf(top, __builtin_fmaf(s[r], runs.r[r >> 3].scale, runs.r[r >> 3].lvs));
+        for (int r = 0; r < 16; r++) top = fmaxf(top, __builtin_fmaf(s[r], runs.r[r >> kRunShift].scale, runs.r[r >> kRunShift].lvs));
         const LanePair both = half_wave_pair(top);
         const float m_new = fmaxf(m_ref, fmaxf(both.lo, both.hi));
         const float alpha = fast_exp2(m_ref - m_new);
@@ -385,28 +413,26 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             if constexpr (kPrecise) (*lo)[j] = static_cast<_Float16>(pe[j] - static_cast<float>(h));
         }
     };
-    auto probabilities_once = [&](const float16v& s, const Runs& runs, Probs& out, float (&sum)[2]) __attribute__((always_inline)) {
+    // sum[a]: of the probabilities of run a
+    auto probabilities_once = [&](const float16v& s, const Runs& runs, Probs& out, float (&sum)[kLaneRuns]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int a = 0; a < kLaneRuns; a++) sum[a] = 0.0f;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const float shift = runs.r[u].lvs - m_ref;
             float pe[8];
-            sum[u] = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                pe[j] = fast_exp2(__builtin_fmaf(s[8 * u + j], runs.r[u].scale, shift));
-                sum[u] += pe[j];
+                const int a = (8 * u + j) >> kRunShift;
+                pe[j] = fast_exp2(__builtin_fmaf(s[8 * u + j], runs.r[a].scale, runs.r[a].lvs - m_ref));
+                sum[a] += pe[j];
             }
             pack(pe, out.hi[u], &out.lo[kPrecise ? u : 0]);
         }
     };
-    auto probabilities = [&](const float16v& s, const Runs& runs, Probs& out) __attribute__((always_inline)) {
-        float sum[2];
-        probabilities_once(s, runs, out, sum);
-        if (__any(!(sum[0] + sum[1] < kProbLimit))) {
-            rebase(s, runs);
-            probabilities_once(s, runs, out, sum);
-        }
-        l_run += sum[0] * runs.r[0].inv + sum[1] * runs.r[1].inv;
+    auto total_of = [&](const float (&sum)[kLaneRuns]) __attribute__((always_inline)) {
+        float t = sum[0] + sum[1];
+        if constexpr (kFine) t += sum[2] + sum[3];
+        return t;
     };
     auto accumulate = [&](uint32_t vbuf, int sub, const Probs& pr) __attribute__((always_inline)) {
         const uint16_t* sv = s_v0 + vbuf * kVTile + 32 * sub * kVPitch;
@@ -432,8 +458,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
 #pragma unroll
         for (int i = 0; i < kRing - 1; i++) ring[i] = k_operand(i);
         float16v c = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-        const float shift[2] = {runs_in.r[0].lvs - m_ref, runs_in.r[1].lvs - m_ref};
-        float psum[2] = {0.0f, 0.0f};
+        float shift[kLaneRuns], psum[kLaneRuns];
+#pragma unroll
+        for (int a = 0; a < kLaneRuns; a++) {
+            shift[a] = runs_in.r[a].lvs - m_ref;
+            psum[a] = 0.0f;
+        }
         float pe[16];
         uint32_t pw[8], pl[kPrecise ? 8 : 1];
         float tn = __builtin_fmaf(s_in[0], runs_in.r[0].scale, shift[0]);
@@ -448,10 +478,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         };
         auto softmax_step = [&](int e) __attribute__((always_inline)) {
             pe[e] = fast_exp2(tn);
-            if (e < 15) tn = __builtin_fmaf(s_in[e + 1], runs_in.r[(e + 1) >> 3].scale, shift[(e + 1) >> 3]);
-            if (e > 0) psum[(e - 1) >> 3] += pe[e - 1];
+            if (e < 15) tn = __builtin_fmaf(s_in[e + 1], runs_in.r[(e + 1) >> kRunShift].scale, shift[(e + 1) >> kRunShift]);
+            if (e > 0) psum[(e - 1) >> kRunShift] += pe[e - 1];
             if (e > 0 && (e & 1) == 0) finish(e / 2 - 1);
-            asm volatile("" : "+v"(pe[e]), "+v"(tn), "+v"(psum[0]), "+v"(psum[1]));
+            asm volatile("" : "+v"(pe[e]), "+v"(tn), "+v"(psum[e >> kRunShift]));
+            if (e > 0) asm volatile("" : "+v"(psum[(e - 1) >> kRunShift]));
         };
         constexpr int kPer = 16 / kPhase;
         auto vector_work = [&](int step) __attribute__((always_inline)) {
@@ -469,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         }
 #pragma unroll
         for (int i = 0; i < kRing - 1; i++) ring[i] = v_operand(i);
-        apply_mask(key0_q, kRows == kExContiguous ? 3u : runs_of(it_q, sub_q).bits, c);  // rare
+        apply_mask(key0_q, kRows == kExContiguous ? kAllRuns : runs_of(it_q, sub_q).bits, c);  // rare
 #pragma unroll
         for (int i = 0; i < 2 * kBlocks; i++) {
             if (i + kRing - 1 < 2 * kBlocks) ring[(i + kRing - 1) % kRing] = v_operand(i + kRing - 1);
@@ -479,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             vector_work(kSteps + i);
             __builtin_amdgcn_sched_barrier(0);
         }
-        psum[1] += pe[15];
+        psum[kLaneRuns - 1] += pe[15];
         finish(7);
         p_out.hi[0] = ex_half8(uint4v{pw[0], pw[1], pw[2], pw[3]});
         p_out.hi[1] = ex_half8(uint4v{pw[4], pw[5], pw[6], pw[7]});
@@ -487,11 +518,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             p_out.lo[0] = ex_half8(uint4v{pl[0], pl[1], pl[2], pl[3]});
             p_out.lo[1] = ex_half8(uint4v{pl[4], pl[5], pl[6], pl[7]});
         }
-        if (__any(!(psum[0] + psum[1] < kProbLimit))) {  // rare: the reference has to move, redo the sub-tile
+        if (__any(!(total_of(psum) < kProbLimit))) {  // rare: the reference has to move, redo the sub-tile
             rebase(s_in, runs_in);
             probabilities_once(s_in, runs_in, p_out, psum);
         }
-        l_run += psum[0] * runs_in.r[0].inv + psum[1] * runs_in.r[1].inv;
+#pragma unroll
+        for (int a = 0; a < kLaneRuns; a++) l_run += psum[a] * runs_in.r[a].inv;
         s_out = c;
     };
 
@@ -513,18 +545,23 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         // ---- prologue: in LDS K of the first two tiles and V of the first, in flight K of the third and fourth and V of
         // the second and third, and the rows of the first 64
         Piece a, b;
-        Plan cur = plan_rows(0, plan_entry(0));
-        int32_t next_entry = 0;
+        Plan cur = plan_rows(0, plan_entries(0));
+        Entries next_entries = {};
         Plan next = cur;
-        auto row_of = [&](uint32_t j) __attribute__((always_inline)) { return uint32_t(__builtin_amdgcn_readlane(int(cur.row), int(j % kPlan))); };
-        const uint32_t o0 = row_of(0), o1 = row_of(1), o2 = row_of(2), o3 = row_of(3);
+        auto row_of = [&](uint32_t j) __attribute__((always_inline)) -> At {
+            At at;
+#pragma unroll
+            for (int f = 0; f < kPieceRuns; f++) at.row[f] = uint32_t(__builtin_amdgcn_readlane(int(cur.row[f]), int(j % kPlan)));
+            return at;
+        };
+        const At o0 = row_of(0), o1 = row_of(1), o2 = row_of(2), o3 = row_of(3);
         load_k(o0, a);
         load_v(o0, a);
         load_k(o1, b);
         plan_runs(cur, 0);
         plan_runs(cur, 1);  // (tiles behind the last, which are masked, find valid numbers)
         store_k(0, a);
-        store_v(0, t_begin, o0 >> 31, a);
+        store_v(0, t_begin, o0, a);
         store_k(1, b);
         __builtin_amdgcn_sched_barrier(0);
         load_k(o2, a);
@@ -533,8 +570,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         load_k(o3, b);
         load_v(o2, b);
         __builtin_amdgcn_sched_barrier(0);
-        uint32_t at_v = o3;                   // of the tile whose V is loaded next
-        uint32_t at_v1 = o1, at_v2 = o2;      // of those whose V is in flight: stored next, and the one after
+        At at_v = o3;                // of the tile whose V is loaded next
+        At at_v1 = o1, at_v2 = o2;  // of those whose V is in flight: stored next, and the one after
         __syncthreads();
 
         float16v s0, s1;
@@ -552,12 +589,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         // (the first iteration's second product, of nothing, reads the first tile's V: whatever it holds, every row sees it)
         uint32_t vb_prev = 0, vb_cur = 0, vb_store = 1;
         auto staging = [&](uint32_t it, Piece& piece, int part) __attribute__((always_inline)) {
-            if (part == 0) store_k(kb_store, piece);                      // K of tile it + 2
-            if (part == 2) store_v(vb_store, it + 1, at_v1 >> 31, piece); // V of tile it + 1
+            if (part == 0) store_k(kb_store, piece);                  // K of tile it + 2
+            if (part == 2) store_v(vb_store, it + 1, at_v1, piece);  // V of tile it + 1
             if (part == 4) {  // K of it + 4, V of it + 3
                 const uint32_t j = it + 4 - t_begin;
                 if (j % kPlan == 0) cur = next;
-                const uint32_t at_k = row_of(j);
+                const At at_k = row_of(j);
                 load_k(at_k, piece);
                 load_v(at_v, piece);
                 at_v1 = at_v2;
@@ -567,8 +604,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             if (part == 5) {  // the next 64 tiles, in three steps a few tiles apart
                 const uint32_t j = it + 4 - t_begin, block = j / kPlan + 1;
                 if (t_begin + block * kPlan < n_tiles) {
-                    if (j % kPlan == 32) next_entry = plan_entry(block);
-                    else if (j % kPlan == 40) next = plan_rows(block, next_entry);
+                    if (j % kPlan == 32) next_entries = plan_entries(block);
+                    else if (j % kPlan == 40) next = plan_rows(block, next_entries);
                     else if (j % kPlan == 48) plan_runs(next, block & 1);
                 }
             }
@@ -774,13 +811,15 @@ template <bool kQF32, bool kPrecise, bool kF8, int kRows, int kD>
 int launch_one(const KvParams& p, dim3 grid) {
     auto kernel = kv_tiles_kernel<kQF32, kPrecise, kF8, kRows, kD>;
     static bool configured[kMaxDevices];
-    if (int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(kernel), Shape<kD>::kLdsBytes, configured)) return rc;
-    kernel<<<grid, dim3(kThreads), Shape<kD>::kLdsBytes, ctx().stream>>>(p);
+    if (int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(kernel), Shape<kD, kRows>::kLdsBytes, configured)) return rc;
+    kernel<<<grid, dim3(kThreads), Shape<kD, kRows>::kLdsBytes, ctx().stream>>>(p);
     return launch_status();
 }
 template <bool kQF32, bool kPrecise, int kD>
 int launch_cache(const KvParams& p, dim3 grid, bool f8, int rows) {
-    if (f8) return launch_one<kQF32, kPrecise, true, kExPaged16, kD>(p, grid);
+    if (f8 && rows == kExPaged16) return launch_one<kQF32, kPrecise, true, kExPaged16, kD>(p, grid);
+    if (f8) return launch_one<kQF32, kPrecise, true, kExPaged4, kD>(p, grid);
+    if (rows == kExPaged4) return launch_one<kQF32, kPrecise, false, kExPaged4, kD>(p, grid);
     if (rows == kExPaged16) return launch_one<kQF32, kPrecise, false, kExPaged16, kD>(p, grid);
     return launch_one<kQF32, kPrecise, false, kExContiguous, kD>(p, grid);
 }
@@ -794,7 +833,9 @@ int launch_types(const KvParams& p, dim3 grid, bool q_f32, bool f8, int rows) {
 
 }  // namespace
 
-int launch_kv_tiles(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const ScratchSource& scratch) {
+int launch_kv_tiles(KvParams p, const KvCall& call, bool q_f32, int rows, const ScratchSource& scratch) {
+    const uint32_t D = call.head_dim;
+    const bool f8 = call.f8;
     const uint64_t n_rows = uint64_t(p.seq_q) * p.group;
     if (n_rows >= (1ull << 31)) return GRANITE_HIP_EINVAL;
     p.q_tiles = uint32_t((n_rows + kBM - 1) / kBM);
@@ -804,13 +845,8 @@ int launch_kv_tiles(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const
     // zero of a zero one, go to Q
     p.q_sign = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
     p.scale_log2 = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
-    const uint32_t cus = ctx().compute_units > 0 ? uint32_t(ctx().compute_units) : 256u;
     const uint64_t wgs = uint64_t(p.q_tiles) * p.num_kv_heads;
-    // tiles of a workgroup: the window's, those its rows' positions add to it, the sinks'
-    const uint64_t keys = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + kBM / p.group) : p.max_tokens;
-    const uint32_t tiles = uint32_t((keys + kBN - 1) / kBN);
-    p.n_splits = 1;
-    if (wgs < cus) p.n_splits = min(min(uint32_t((cus + wgs - 1) / wgs), max(tiles / 4, 1u)), 64u);
+    p.n_splits = kv_tiles_cut(call).pieces;
     const size_t slots = p.n_splits > 1 ? size_t(p.n_splits) * p.num_kv_heads * n_rows : 0;
     const size_t need = slots * (D + 2) * sizeof(float);
     if (scratch.query) {

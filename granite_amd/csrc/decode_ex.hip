@@ -10,8 +10,7 @@ namespace {
 
 constexpr uint32_t kRowWaves = 8;
 constexpr uint32_t kDirectTokens = 768;
-constexpr uint32_t kStreamRows = 320, kStreamRowsHalf = 160;  // float, half results
-constexpr uint32_t kFewRows = 32, kFewRowsTokens = 6144;
+constexpr uint32_t kStreamRows = 1280;  // most rows of a KV head that the persistent kernel takes
 
 // One workgroup per (run of 16 query rows, KV head, sequence, key split).  A row is a (query, head of
 // the KV head's group) pair, row r = query * group + head, so a decode step's group, a few draft tokens and a
@@ -156,18 +155,29 @@ int launch_rows_cache(const KvParams& p, dim3 grid, uint32_t D, bool f8, int row
     return launch_rows_dim<kQF32, false, kExPagedAny>(p, grid, D);
 }
 
+KvCall call_of(const KvParams& p, uint32_t D, bool q_f32, bool f8, int rows) {
+    KvCall c{};
+    c.rows = uint64_t(p.seq_q) * p.group;
+    c.lists = p.num_kv_heads * p.batch;
+    c.queries = p.seq_q;
+    c.group = p.group;
+    c.head_dim = D;
+    c.start_pos = p.start_pos;
+    c.length = p.causal && !p.decode ? uint32_t(min(uint64_t(p.max_tokens), uint64_t(p.start_pos) + p.seq_q)) : p.max_tokens;
+    c.window_keys = p.window ? uint64_t(p.window) + p.sinks : 0;
+    c.causal = p.causal && !p.decode;
+    c.f8 = f8;
+    c.paged_runs = rows != kExPagedAny;
+    c.wide = q_f32 || p.out_f32;
+    c.cus = ctx().compute_units > 0 ? uint32_t(ctx().compute_units) : 256u;
+    return c;
+}
+
 // The row kernel for any launch.
 int launch_rows(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const ScratchSource& scratch) {
     const uint32_t row_tiles = uint32_t((uint64_t(p.seq_q) * p.group + 15) / 16);
     if (p.num_kv_heads > 65535u || p.batch > 65535u || p.seq_q > 65535u) return GRANITE_HIP_EINVAL;
-    const uint32_t cus = ctx().compute_units > 0 ? uint32_t(ctx().compute_units) : 256u;
-    const uint64_t wgs = uint64_t(row_tiles) * p.num_kv_heads * p.batch;
-    // keys a row can see, in tiles
-    const uint32_t keys = p.window ? uint32_t(min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks)) : p.max_tokens;
-    const uint32_t tiles = (keys + 63) / 64;
-    uint32_t splits = wgs < cus ? uint32_t((cus + wgs - 1) / wgs) : 1u;
-    splits = min(splits, max(tiles / kRowWaves, 1u));
-    p.n_splits = min(splits, 64u);
+    p.n_splits = kv_rows_cut(call_of(p, D, q_f32, f8, rows)).pieces;
     if (uint64_t(row_tiles) * p.n_splits > 0x7FFFFFFFull) return GRANITE_HIP_EINVAL;
     const size_t slots = p.n_splits > 1 ? size_t(p.n_splits) * p.batch * p.num_heads * p.seq_q : 0;
     const size_t need = slots * (D + 2) * sizeof(float);
@@ -345,20 +355,21 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     p.causal = a.mask_mode == GRANITE_HIP_MASK_CAUSAL;
     p.start_pos = a.start_pos;
     p.scale_log2 = a.scale * kExLog2e;
-    // Few rows of 8-bit pools: the persistent kernel of the decode step, 16 rows in the place of a head's group.  A draft's
-    // worth of them on few keys is quicker on the row kernel (8 queries of 32 heads over 8 KV heads, half results: 200 keys
-    // 8.7 us against 11.7, 4096 keys 16.8 against 20.0; 32768 keys 36.5 against 34.0).
-    const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3;
-    const uint64_t n_rows = uint64_t(a.seq_q) * p.group;
+    // The quickest of three (kv_choice.h): the row kernel, which takes anything; the tiles kernel; for 8-bit pools the persistent
+    // kernel of the decode step, 16 rows in the place of a head's group.
+    const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3, q_f32 = a.q_dtype == GRANITE_HIP_F32;
+    const KvCall call = call_of(p, D, q_f32, f8, rows);
+    int tile_rows = rows;
+    if (rows == kExPagedAny && a.block_size % 4 == 0 && p.row_bytes < (1 << 27)) tile_rows = kExPaged4;
+    const bool tiled = tile_rows != kExPagedAny && call.rows < (1ull << 31);
     const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
-    if (f8 && rows == kExPaged16 && n_rows <= (p.out_f32 ? kStreamRows : kStreamRowsHalf) && (n_rows > kFewRows || seen > kFewRowsTokens)) {
-        const uint32_t tiles = uint32_t((seen + 31) / 32);
-        p.q_groups = uint32_t((n_rows + 15) / 16);
-        if (kv_stream_supports(p, tiles)) return launch_kv_stream(p, D, a.q_dtype == GRANITE_HIP_F32, f8, rows, tiles, scratch);
-    }
-    if (rows != kExPagedAny && n_rows > kFewRows)
-        return launch_kv_tiles(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
-    return launch_rows(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
+    const uint32_t tiles = uint32_t((seen + 31) / 32);
+    p.q_groups = uint32_t((call.rows + 15) / 16);
+    const bool streamed = f8 && rows == kExPaged16 && call.rows <= kStreamRows && kv_stream_supports(p, tiles);
+    const double rows_us = kv_rows_cut(call).us, tiles_us = tiled ? kv_tiles_cut(call).us : INFINITY, stream_us = streamed ? kv_stream_us(call) : INFINITY;
+    if (stream_us < min(rows_us, tiles_us)) return launch_kv_stream(p, D, q_f32, f8, rows, tiles, scratch);
+    if (tiles_us < rows_us) return launch_kv_tiles(p, call, q_f32, tile_rows, scratch);
+    return launch_rows(p, D, q_f32, f8, rows, scratch);
 }
 
 }  // namespace ghip

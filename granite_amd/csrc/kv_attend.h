@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.h"
+#include "kv_choice.h"
 #include "kv_visible.h"
 
 namespace ghip {
@@ -13,8 +14,8 @@ constexpr float kExNegBig = -1.0e30f;
 
 // How token positions map to rows.  Runs of 16 consecutive tokens that start at a multiple of 16 lie in
 // one block when the block size is a multiple of 16: one table entry, one scale and one base address
-// then serve 16 tokens and stay in scalar registers.
-enum : int { kExContiguous = 0, kExPaged16 = 1, kExPagedAny = 2 };
+// then serve 16 tokens and stay in scalar registers.  kExPaged4, runs of 4, is the tiles kernel's only.
+enum : int { kExContiguous = 0, kExPaged16 = 1, kExPagedAny = 2, kExPaged4 = 3 };
 
 struct KvParams {
     const void* q;
@@ -59,8 +60,8 @@ int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint
 constexpr uint32_t kDmaMaxBatch = 2560;
 size_t kv_dma_lds_bytes(uint32_t D, uint32_t batch);
 int launch_kv_dma(const KvParams& p, uint32_t D, bool q_f32, uint32_t per_list, dim3 grid);
-// attention_ex.hip: the tiles kernel.  Block sizes are multiples of 16, or the cache is contiguous.
-int launch_kv_tiles(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const ScratchSource& scratch);
+// attention_ex.hip: the tiles kernel.  Block sizes are multiples of 4, or the cache is contiguous.
+int launch_kv_tiles(KvParams p, const KvCall& call, bool q_f32, int rows, const ScratchSource& scratch);
 
 #if defined(__HIPCC__)
 

@@ -16,12 +16,20 @@ ROOT = Path(__file__).resolve().parent.parent
 P = 1 << 20  # a pointer that is only tested
 
 
-def test_visible_tiles_against_single_keys(tmp_path):
-    exe = tmp_path / "kv_visible_test"
+def host_test(tmp_path, name):
+    exe = tmp_path / name
     subprocess.run(["g++", "-std=c++20", "-O1", "-Wall", "-Wextra", "-I", str(ROOT / "granite_amd" / "csrc"),
-                    str(ROOT / "granite_amd" / "host" / "tests" / "kv_visible_test.cpp"), "-o", str(exe)], check=True)
+                    str(ROOT / "granite_amd" / "host" / "tests" / f"{name}.cpp"), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True)
     assert out.returncode == 0 and out.stdout.strip().endswith("ok"), out.stdout
+
+
+def test_visible_tiles_against_single_keys(tmp_path):
+    host_test(tmp_path, "kv_visible_test")
+
+
+def test_choice_of_kernel(tmp_path):
+    host_test(tmp_path, "kv_choice_test")
 
 
 def decode(form=(), **changes):
