@@ -9,7 +9,6 @@ namespace ghip {
 namespace {
 
 constexpr uint32_t kRowWaves = 8;
-constexpr uint32_t kDirectTokens = 768;
 constexpr uint32_t kStreamRows = 1280;  // most rows of a KV head that the persistent kernel takes
 
 // One workgroup per (run of 16 query rows, KV head, sequence, key split).  A row is a (query, head of
@@ -299,9 +298,10 @@ int launch_decode_ex(const granite_hip_decode_args& a, const granite_hip_kv_form
     const uint32_t tile = kv_stream_tile(p, f8, rows);
     const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + 2 * tile) : p.max_tokens;
     const uint32_t tiles = uint32_t((seen + tile - 1) / tile);
-    if (tiles * tile > kDirectTokens && kv_stream_supports(p, tiles))
-        return launch_kv_stream(p, D, a.q_dtype == GRANITE_HIP_F32, f8, rows, tiles, scratch);
-    return launch_rows(p, D, a.q_dtype == GRANITE_HIP_F32, f.kv_dtype == GRANITE_HIP_F8E4M3, rows, scratch);
+    const bool q_f32 = a.q_dtype == GRANITE_HIP_F32;
+    const KvCall call = call_of(p, D, q_f32, f8, rows);
+    if (kv_stream_supports(p, tiles) && kv_stream_us(call) < kv_rows_cut(call).us) return launch_kv_stream(p, D, q_f32, f8, rows, tiles, scratch);
+    return launch_rows(p, D, q_f32, f8, rows, scratch);
 }
 
 int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_kv_form& f, const ScratchSource& scratch) {

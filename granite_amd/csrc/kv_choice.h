@@ -1,11 +1,12 @@
-// Which kernel a call with several queries takes over 8-bit pools or through a window, and into how many pieces
-// the keys are cut: estimates in microseconds from the sizes alone, plain arithmetic without HIP.
+// Which kernel a call takes over 8-bit pools or through a window, and into how many pieces the keys are cut: estimates
+// in microseconds from the sizes alone, plain arithmetic without HIP.
 //
 // The three candidates differ in how many query rows share what is read.  The row kernel has 16 a workgroup: little to set
-// up, and every 16 rows read their keys again.  The persistent kernel has 16 a wave and no tail.  The tiles kernel has
-// 256 a workgroup and runs at the rate of the matrix cores, behind a long prologue.  The constants are fits to 160 calls
-// drawn over 2 to 1500 queries, 1 to 16 KV heads, contexts up to 33000 and windows from 1 on, each timed on all three:
-// following the estimates costs 2.4 % over the best of the three (a rule on the number of rows alone: 27 %).
+// up, and every 16 rows read their keys again.  The persistent kernel has 16 a wave, a fixed number of waves and no tail.  The
+// tiles kernel has 256 a workgroup and runs at the rate of the matrix cores, behind a long prologue.  The constants are
+// fits to 160 calls drawn over 2 to 1500 queries, 1 to 16 KV heads, contexts up to 33000 and windows from 1 on, each timed on
+// all three (following the estimates costs 1.7 % over the best of the three on 100 other calls, a rule on the number of
+// rows alone 34 %), and to 150 decode steps of 1 to 64 sequences (0.7 %; by the length of the context alone 4.5 %).
 #pragma once
 
 #include <stdint.h>
@@ -80,10 +81,15 @@ inline KvCut kv_tiles_cut(const KvCall& c) {
     return best;
 }
 
-// Persistent kernel over 8-bit pools: tiles of 32 tokens for 16 rows, eight waves a CU.
+// Persistent kernel: eight waves a CU share the tiles of 16 rows, 32 tokens each or, of an 8-bit pool with a table entry per
+// token, 64.
 inline double kv_stream_us(const KvCall& c) {
-    const double units = double((c.rows + 15) / 16) * c.lists * (kv_keys(c, c.rows) / 32 + 0.5);
-    return 10.0 + std::max(1.0, units / (8.0 * c.cus)) * (c.head_dim == 128 ? 2.6 : 1.6);
+    const bool wide_tile = c.f8 && !c.paged_runs;
+    const uint32_t tokens = wide_tile ? 64 : 32;
+    const double units = double((c.rows + 15) / 16) * c.lists * (kv_keys(c, c.rows) / tokens + 0.5) / (8.0 * c.cus);
+    double unit_us = (c.head_dim == 128 ? 2.6 : 1.6) * (c.f8 ? 1 : 2);
+    if (!c.paged_runs) unit_us = (c.f8 ? 2.0 : 1.0) * (c.head_dim == 128 ? 5.5 : 2.6);
+    return (c.paged_runs ? 9.5 : 11.0) + std::max(1.0, units) * unit_us;
 }
 
 }  // namespace ghip
