@@ -295,12 +295,12 @@ int launch_decode_ex(const granite_hip_decode_args& a, const granite_hip_kv_form
     p.q_groups = (p.group + 15) / 16;
     // Tiles of the longest sequence: its whole length, or its window and sinks and the tiles their ends lie in.
     const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3;
-    const uint32_t tile = kv_stream_tile(p, f8, rows);
+    constexpr uint32_t tile = 32;
     const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + 2 * tile) : p.max_tokens;
     const uint32_t tiles = uint32_t((seen + tile - 1) / tile);
     const bool q_f32 = a.q_dtype == GRANITE_HIP_F32;
     const KvCall call = call_of(p, D, q_f32, f8, rows);
-    if (kv_stream_supports(p, tiles) && kv_stream_us(call) < kv_rows_cut(call).us) return launch_kv_stream(p, D, q_f32, f8, rows, tiles, scratch);
+    if (kv_stream_supports(p, f8, rows, tiles) && kv_stream_us(call) < kv_rows_cut(call).us) return launch_kv_stream(p, D, q_f32, f8, rows, tiles, scratch);
     return launch_rows(p, D, q_f32, f8, rows, scratch);
 }
 
@@ -365,7 +365,7 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
     const uint32_t tiles = uint32_t((seen + 31) / 32);
     p.q_groups = uint32_t((call.rows + 15) / 16);
-    const bool streamed = f8 && rows == kExPaged16 && call.rows <= kStreamRows && kv_stream_supports(p, tiles);
+    const bool streamed = f8 && call.rows <= kStreamRows && kv_stream_supports(p, f8, rows, tiles);
     const double rows_us = kv_rows_cut(call).us, tiles_us = tiled ? kv_tiles_cut(call).us : INFINITY, stream_us = streamed ? kv_stream_us(call) : INFINITY;
     if (stream_us < min(rows_us, tiles_us)) return launch_kv_stream(p, D, q_f32, f8, rows, tiles, scratch);
     if (tiles_us < rows_us) return launch_kv_tiles(p, call, q_f32, tile_rows, scratch);

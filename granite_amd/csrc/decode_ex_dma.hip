@@ -494,7 +494,7 @@ template <bool kQF32, int kD, uint32_t kPer, bool kMulti>
 int launch_rows_of(const KvParams& p, dim3 grid, size_t lds) {
     auto kernel = kv_dma_kernel<kQF32, kD, kPer, kMulti>;
     static bool configured[kMaxDevices];
-    if (int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(kernel), kv_dma_lds_bytes(kD, kDmaMaxBatch), configured)) return rc;
+    if (int rc = raise_dynamic_lds_limit(reinterpret_cast<const void*>(kernel), kv_dma_lds_bytes(kD, kStreamMaxBatch), configured)) return rc;
     kernel<<<grid, dim3(kWaves * kWave), lds, ctx().stream>>>(p);
     return launch_status();
 }

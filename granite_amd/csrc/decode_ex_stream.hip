@@ -1,5 +1,7 @@
-// Decode over 8-bit pools and windowed caches, persistent form: one workgroup per CU walks an equal share of the
-// visible key tiles of the whole batch.
+// Decode through a window over half caches, persistent form: one workgroup per CU walks an equal share of the visible
+// key tiles of the whole batch; the joining of its pieces, and of those of decode_ex_dma.hip, which does the same over
+// 8-bit pools.  Contiguous caches, and pools whose blocks are multiples of 16 tokens: where every token has a table entry of
+// its own the row kernel is as quick (64 sequences of 8192 over 8-bit blocks of 20: 227 us against 306).
 //
 // The flat list is ordered (sequence, list head, tile): the tiles are those of kv_visible.h, so under a window a long
 // sequence contributes its window and its sinks and nothing else.  Workers take equal contiguous ranges of the list; one that
@@ -15,8 +17,7 @@
 // worker is a wave.
 //
 // Inside a wave the K and V of the next tile are in flight while one is computed (16 KiB; 128 KiB per CU); its
-// block-table entries are a tile further ahead, and the scales, which need the entries, are requested just before
-// the K and V they belong to.  All loads are unconditional: a load inside a branch would make the
+// block-table entries are a tile further ahead.  All loads are unconditional: a load inside a branch would make the
 // compiler wait for every outstanding one at the join.
 #include "common.h"
 #include "kv_attend.h"
@@ -26,12 +27,11 @@ namespace {
 
 constexpr uint32_t kWaves = 8;
 constexpr uint32_t kPlanHeader = 4;
-constexpr uint32_t kMaxPrefix = 7680;  // lengths and prefix sums in LDS: 60 KiB
 
-template <bool kQF32, bool kF8, int kRows, int kD, uint32_t kPer>
+template <bool kQF32, int kRows, int kD, uint32_t kPer>
 __global__ void __launch_bounds__(kWaves* kWave, 2) kv_stream_kernel(KvParams p) {
-    using T = Tile<kF8, kRows, kD>;
-    using R = Rows16<kQF32, kF8, kD>;
+    using T = Tile<false, kRows, kD>;
+    using R = Rows16<kQF32, false, kD>;
     const uint32_t lane = threadIdx.x & 63, wave = ex_uniform(threadIdx.x >> 6);
     const uint32_t n = lane & 15, g = lane >> 4;
     const uint32_t worker = blockIdx.x * (kWaves / kPer) + wave / kPer;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_stream_kernel(KvParams p)
         const uint32_t len = of_unit(d_len, i), tok0 = of_unit(d_tok, i);
         const VisibleTiles seen = seen_of(len);
         const bool masked = T::needs_mask(p, rows, tok0, seen.lo, len);
-        attend_tile<kQF32, kF8, kRows, kD, false>(p, tile, rows, tok0, seen, seen.lo, len, masked, st, lane);
+        attend_tile<kQF32, false, kRows, kD, false>(p, tile, rows, tok0, seen, seen.lo, len, masked, st, lane);
     };
     auto flush = [&](uint32_t i, R& st) __attribute__((always_inline)) {
         const uint32_t vh = head_at(i), lh = of_unit(d_lh, i) & 0x7FFFFFFFu;
@@ -272,37 +272,25 @@ __global__ void __launch_bounds__(kD* kJoin) kv_stream_merge_kernel(KvParams p) 
             l == 0.0f ? -INFINITY : (mx + __builtin_amdgcn_logf(l)) * kExLn2;
 }
 
-template <bool kQF32, bool kF8, int kRows, int kD>
+template <bool kQF32, int kRows, int kD>
 void launch_shape(const KvParams& p, uint32_t per_list, dim3 grid, size_t lds) {
     const dim3 block(kWaves * kWave);
     hipStream_t st = ctx().stream;
-    if (per_list == 8) kv_stream_kernel<kQF32, kF8, kRows, kD, 8><<<grid, block, lds, st>>>(p);
-    else if (per_list == 4) kv_stream_kernel<kQF32, kF8, kRows, kD, 4><<<grid, block, lds, st>>>(p);
-    else if (per_list == 2) kv_stream_kernel<kQF32, kF8, kRows, kD, 2><<<grid, block, lds, st>>>(p);
-    else kv_stream_kernel<kQF32, kF8, kRows, kD, 1><<<grid, block, lds, st>>>(p);
+    if (per_list == 8) kv_stream_kernel<kQF32, kRows, kD, 8><<<grid, block, lds, st>>>(p);
+    else if (per_list == 4) kv_stream_kernel<kQF32, kRows, kD, 4><<<grid, block, lds, st>>>(p);
+    else if (per_list == 2) kv_stream_kernel<kQF32, kRows, kD, 2><<<grid, block, lds, st>>>(p);
+    else kv_stream_kernel<kQF32, kRows, kD, 1><<<grid, block, lds, st>>>(p);
 }
-template <bool kQF32, int kD>
-void launch_cache(const KvParams& p, uint32_t per_list, dim3 grid, size_t lds, bool f8, int rows) {
-    if (f8 && rows == kExPaged16) launch_shape<kQF32, true, kExPaged16, kD>(p, per_list, grid, lds);
-    else if (f8) launch_shape<kQF32, true, kExPagedAny, kD>(p, per_list, grid, lds);
-    else if (rows == kExContiguous) launch_shape<kQF32, false, kExContiguous, kD>(p, per_list, grid, lds);
-    else if (rows == kExPaged16) launch_shape<kQF32, false, kExPaged16, kD>(p, per_list, grid, lds);
-    else launch_shape<kQF32, false, kExPagedAny, kD>(p, per_list, grid, lds);
-}
-
-}  // namespace
-
-uint32_t kv_stream_tile(const KvParams& p, bool f8, int rows) {
-    if (!f8) return 32;
-    return rows == kExPaged16 && p.batch <= kDmaMaxBatch ? 32 : 64;
+template <int kD>
+void launch_types(const KvParams& p, uint32_t per_list, dim3 grid, size_t lds, bool q_f32, int rows) {
+    if (q_f32 && rows == kExContiguous) launch_shape<true, kExContiguous, kD>(p, per_list, grid, lds);
+    else if (q_f32) launch_shape<true, kExPaged16, kD>(p, per_list, grid, lds);
+    else if (rows == kExContiguous) launch_shape<false, kExContiguous, kD>(p, per_list, grid, lds);
+    else launch_shape<false, kExPaged16, kD>(p, per_list, grid, lds);
 }
 
-bool kv_stream_supports(const KvParams& p, uint32_t tiles_per_seq) {
-    const uint64_t units = uint64_t(p.batch) * tiles_per_seq * p.num_kv_heads * p.q_groups;
-    return p.batch + 1 <= kMaxPrefix && units < (1ull << 31) && p.num_heads <= 0x7FFFFFFFu && p.batch <= 65535u;
-}
-
-int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t tiles_per_seq, const ScratchSource& scratch) {
+// At most kStreamMaxBatch sequences, whose lengths and prefix sums lie in LDS.
+int launch_part(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t tiles_per_seq, const ScratchSource& scratch) {
     const uint32_t cus = ctx().compute_units > 0 ? uint32_t(ctx().compute_units) : 256u;
     const uint32_t vheads = p.num_kv_heads * p.q_groups;
     const uint32_t per_list = vheads % 8 == 0 ? 8 : vheads % 4 == 0 ? 4 : vheads % 2 == 0 ? 2 : 1;
@@ -325,21 +313,19 @@ int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint
     p.part_ml = p.part_o + slots * D;
     const size_t lds = (2 * size_t(p.batch) + 1) * sizeof(uint32_t);
     {
-        KernelTimerScope timer("decode_ex");
+        KernelTimerScope timer(p.decode ? "decode_ex" : "attention_ex");
         const dim3 grid(cus);
-        if (kv_stream_tile(p, f8, rows) == 32 && f8) {
+        if (f8) {
             if (int rc = launch_kv_dma(p, D, q_f32, per_list, grid)) return rc;
         } else if (D == 128) {
-            if (q_f32) launch_cache<true, 128>(p, per_list, grid, lds, f8, rows);
-            else launch_cache<false, 128>(p, per_list, grid, lds, f8, rows);
+            launch_types<128>(p, per_list, grid, lds, q_f32, rows);
         } else {
-            if (q_f32) launch_cache<true, 64>(p, per_list, grid, lds, f8, rows);
-            else launch_cache<false, 64>(p, per_list, grid, lds, f8, rows);
+            launch_types<64>(p, per_list, grid, lds, q_f32, rows);
         }
     }
     if (int rc = launch_status()) return rc;
     {
-        KernelTimerScope timer("decode_ex_merge");
+        KernelTimerScope timer(p.decode ? "decode_ex_merge" : "attention_ex_merge");
         const dim3 grid(p.seq_q * p.num_heads, p.batch);
         const bool few = size_t(p.batch) * lists * 16 <= p.workers;  // 16 pieces a segment or more if all are as long
         hipStream_t st = ctx().stream;
@@ -349,6 +335,29 @@ int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint
         else kv_stream_merge_kernel<64, 1><<<grid, dim3(64), 0, st>>>(p);
     }
     return launch_status();
+}
+
+}  // namespace
+
+bool kv_stream_supports(const KvParams& p, bool f8, int rows, uint32_t tiles_per_seq) {
+    if (rows == kExPagedAny || (f8 && rows == kExContiguous)) return false;
+    const uint64_t units = uint64_t(min(p.batch, kStreamMaxBatch)) * tiles_per_seq * p.num_kv_heads * p.q_groups;
+    return units < (1ull << 31) && uint64_t(p.seq_q) * p.num_heads <= 0x7FFFFFFFu;
+}
+
+int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t tiles_per_seq, const ScratchSource& scratch) {
+    const uint32_t batch = p.batch;
+    for (uint32_t b = 0; b < batch; b += kStreamMaxBatch) {  // (the parts follow each other on the stream and may share the workspace)
+        p.batch = min(batch - b, kStreamMaxBatch);
+        if (int rc = launch_part(p, D, q_f32, f8, rows, tiles_per_seq, scratch)) return rc;
+        if (scratch.query) break;  // the first part is the largest
+        p.q = static_cast<const char*>(p.q) + size_t(p.batch) * p.q_batch * (q_f32 ? 4 : 2);
+        p.out = static_cast<char*>(p.out) + size_t(p.batch) * p.out_batch * (p.out_f32 ? 4 : 2);
+        if (p.tables) p.tables += size_t(p.batch) * p.max_blocks;
+        if (p.seq_lens) p.seq_lens += p.batch;
+        if (p.lse) p.lse += size_t(p.batch) * p.lse_batch;
+    }
+    return GRANITE_HIP_OK;
 }
 
 }  // namespace ghip

@@ -51,13 +51,11 @@ struct KvParams {
     float q_sign;  // tiles kernel: 1, -1 or 0, taken into Q
 };
 
-// decode_ex_stream.hip: the persistent decode kernel.  tiles_per_seq: most tiles a sequence can have to visit.
-uint32_t kv_stream_tile(const KvParams& p, bool f8, int rows);  // tokens of a tile of the kernel that will run
-bool kv_stream_supports(const KvParams& p, uint32_t tiles_per_seq);
+// decode_ex_stream.hip: the persistent kernels, tiles of 32 tokens.  tiles_per_seq: most tiles a sequence can have to visit.
+constexpr uint32_t kStreamMaxBatch = 2560;  // sequences of a launch: larger batches go in parts
+bool kv_stream_supports(const KvParams& p, bool f8, int rows, uint32_t tiles_per_seq);
 int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t tiles_per_seq, const ScratchSource& scratch);
-// decode_ex_dma.hip: the same over 8-bit pools with blocks of multiples of 16 tokens, tiles of 32 tokens, through
-// LDS; p as launch_kv_stream has it, for the batches whose lengths fit LDS beside the tiles.
-constexpr uint32_t kDmaMaxBatch = 2560;
+// decode_ex_dma.hip: the one over 8-bit pools, through LDS; p as launch_kv_stream has it.
 size_t kv_dma_lds_bytes(uint32_t D, uint32_t batch);
 int launch_kv_dma(const KvParams& p, uint32_t D, bool q_f32, uint32_t per_list, dim3 grid);
 // attention_ex.hip: the tiles kernel.  Block sizes are multiples of 4, or the cache is contiguous.

@@ -52,16 +52,17 @@ inline double kv_join_us(const KvCall& c, uint32_t pieces) {
 }
 
 // Row kernel: eight waves take tiles of 64 tokens in turn, 3 us each (4.5 where every token has its own table entry) as long
-// as memory gives 4.4 TB/s.
+// as memory gives 4.4 TB/s (5.2 where rows are 256 bytes), of which a CU gets at most 1/150.
 inline KvCut kv_rows_cut(const KvCall& c) {
     const double workgroups = double((c.rows + 15) / 16) * c.lists, tiles = std::ceil(kv_keys(c, 16) / 64);
     const double tile_us = c.paged_runs ? 3.0 : c.f8 ? 4.5 : 3.5;
-    const double memory_us = workgroups * tiles * 128.0 * c.head_dim * (c.f8 ? 1 : 2) / 4.4e6;
+    const double row_bytes = double(c.head_dim) * (c.f8 ? 1 : 2);
+    const double memory_us = workgroups * tiles * 128.0 * row_bytes / (row_bytes >= 256 ? 5.2e6 : 4.4e6);
     KvCut best{1, 0.0};
     const uint32_t most = uint32_t(std::min(std::max(tiles / 8, 1.0), 64.0));
     for (uint32_t n = 1; n <= most && (n == 1 || workgroups * n <= c.cus); n++) {
         const double busy = kv_rounds(workgroups * n, c.cus) * (1.5 + std::max(1.0, tiles / (8.0 * n)) * tile_us);
-        const double us = 4.0 + std::max(memory_us, busy) + kv_join_us(c, n);
+        const double us = 4.0 + std::max(memory_us * std::max(1.0, 0.6 * c.cus / (workgroups * n)), busy) + kv_join_us(c, n);
         if (n == 1 || us < best.us) best = {n, us};
     }
     return best;
@@ -81,15 +82,11 @@ inline KvCut kv_tiles_cut(const KvCall& c) {
     return best;
 }
 
-// Persistent kernel: eight waves a CU share the tiles of 16 rows, 32 tokens each or, of an 8-bit pool with a table entry per
-// token, 64.
+// Persistent kernel (blocks of multiples of 16 tokens, or a contiguous cache): eight waves a CU share the tiles of 16 rows
+// and 32 tokens.
 inline double kv_stream_us(const KvCall& c) {
-    const bool wide_tile = c.f8 && !c.paged_runs;
-    const uint32_t tokens = wide_tile ? 64 : 32;
-    const double units = double((c.rows + 15) / 16) * c.lists * (kv_keys(c, c.rows) / tokens + 0.5) / (8.0 * c.cus);
-    double unit_us = (c.head_dim == 128 ? 2.6 : 1.6) * (c.f8 ? 1 : 2);
-    if (!c.paged_runs) unit_us = (c.f8 ? 2.0 : 1.0) * (c.head_dim == 128 ? 5.5 : 2.6);
-    return (c.paged_runs ? 9.5 : 11.0) + std::max(1.0, units) * unit_us;
+    const double units = double((c.rows + 15) / 16) * c.lists * (kv_keys(c, c.rows) / 32 + 0.5) / (8.0 * c.cus);
+    return 9.5 + std::max(1.0, units) * (c.f8 ? (c.head_dim == 128 ? 2.6 : 1.6) : (c.head_dim == 128 ? 6.0 : 3.3));
 }
 
 }  // namespace ghip

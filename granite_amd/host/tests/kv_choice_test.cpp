@@ -61,6 +61,24 @@ int main() {
                    "case %d window %u", i, window);
         EXPECT(kv_rows_cut(call(4, 500, 32, 8, dim, f8, runs, wide, 0)).us < kv_tiles_cut(call(4, 500, 32, 8, dim, f8, runs, wide, 0)).us, "case %d", i);
     }
+    // decode steps: sequences, heads, KV heads, head size, tokens a sequence may have, window and sinks, 8-bit
+    struct Step {
+        uint32_t batch, heads, kv_heads, dim, capacity, window_keys;
+        bool f8, streamed;
+    };
+    for (const Step& s : {Step{24, 32, 8, 128, 3008, 0, true, true}, Step{24, 16, 16, 64, 2944, 0, true, true}, Step{40, 28, 4, 128, 3008, 0, true, true},
+                          Step{60, 48, 1, 64, 4064, 0, true, true}, Step{30, 40, 5, 128, 3008, 0, true, true}, Step{40, 34, 2, 128, 4096, 0, true, true},
+                          Step{24, 32, 8, 128, 3008, 2537, true, true}, Step{24, 16, 16, 128, 3024, 2004, true, true}, Step{24, 16, 16, 64, 2528, 0, true, true},
+                          Step{24, 16, 16, 64, 3024, 2504, true, true}, Step{24, 16, 16, 64, 3024, 2504, false, true}, Step{24, 16, 16, 64, 3024, 2004, false, true},
+                          Step{16, 16, 8, 128, 4064, 4000, false, true}, Step{16, 16, 8, 128, 4064, 2637, false, true}, Step{16, 24, 24, 64, 4064, 2637, false, true},
+                          Step{16, 24, 24, 64, 4064, 4000, false, true}, Step{1, 32, 16, 128, 16000, 9000, false, true}, Step{1, 48, 48, 64, 16000, 9000, false, true},
+                          Step{1, 32, 8, 128, 512, 0, true, false}, Step{4, 32, 8, 128, 256, 0, true, false}, Step{16, 32, 8, 128, 64, 0, true, false}}) {
+        KvCall c = call(1, 0, s.heads, s.kv_heads, s.dim, s.f8, true, true, s.window_keys);
+        c.lists = s.batch * s.kv_heads;
+        c.length = s.capacity;
+        c.causal = false;
+        EXPECT((kv_stream_us(c) < kv_rows_cut(c).us) == s.streamed, "%u sequences of %u, %u heads of %u, window %u: %f against %f", s.batch, s.capacity, s.kv_heads, s.dim, s.window_keys, kv_stream_us(c), kv_rows_cut(c).us);
+    }
     EXPECT(kv_stream_us(call(4, 32768, 32, 8, 128, true, true, false, 0)) < kv_rows_cut(call(4, 32768, 32, 8, 128, true, true, false, 0)).us, "a draft");
     if (failures) {
         std::printf("%d failures\n", failures);
