@@ -175,8 +175,8 @@ KvCall call_of(const KvParams& p, uint32_t D, bool q_f32, bool f8, int rows) {
 // The row kernel for any launch.
 int launch_rows(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, const ScratchSource& scratch) {
     const uint32_t row_tiles = uint32_t((uint64_t(p.seq_q) * p.group + 15) / 16);
-    if (p.num_kv_heads > 65535u || p.batch > 65535u || p.seq_q > 65535u) return GRANITE_HIP_EINVAL;
-    p.n_splits = kv_rows_cut(call_of(p, D, q_f32, f8, rows)).pieces;
+    if (p.num_kv_heads > 65535u || p.batch > 65535u) return GRANITE_HIP_EINVAL;
+    p.n_splits = p.seq_q > 65535u ? 1u : kv_rows_cut(call_of(p, D, q_f32, f8, rows)).pieces;  // (the merge's grid has a row per query)
     if (uint64_t(row_tiles) * p.n_splits > 0x7FFFFFFFull) return GRANITE_HIP_EINVAL;
     const size_t slots = p.n_splits > 1 ? size_t(p.n_splits) * p.batch * p.num_heads * p.seq_q : 0;
     const size_t need = slots * (D + 2) * sizeof(float);

@@ -128,3 +128,25 @@ def test_prefill_few_rows_many_keys(gpu, n, start, bs, hq, hkv, d, q_dtype, out_
     run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype)
     run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype, 6190, 5)
     run_prefill(gpu, cache, n, start, hq, q_dtype, out_dtype, 6200 + n // 2, 0)   # the first queries'
+
+
+@pytest.mark.parametrize("kv,bs", [(F8E4M3, 5), (F8E4M3, 16), (F16, 7), (F16, 12)])
+def test_prefill_seventy_thousand_queries(gpu, kv, bs):
+    say(f"prefill 70000 queries kv={kv} bs={bs}")
+    n, d, start = 70000, 64, 11
+    rng = np.random.default_rng(bs)
+    cache = Shared(rng, 1, -(-(start + n) // bs), 50, bs, 1, d, kv)
+    q = rng.standard_normal((n, 1, d), dtype=np.float32).astype(np.float16)
+    out, dq = dev(np.full(q.shape, 7.0, np.float16)), dev(q)
+    lse = dev(np.full((1, n), 7.0, np.float32))
+    gpu.attention_ex(q=dq, q_dtype=F16, q_tok_stride=d, q_head_stride=d, out=out, out_dtype=F16, out_tok_stride=d, out_head_stride=d,
+                     seq_q=n, num_heads=1, scale=d ** -0.5, cache_len=start + n, block_table=cache.dev[4], mask_mode=MASK_CAUSAL,
+                     start_pos=start, lse=lse, window=33, num_sinks=2, **cache.kwargs())
+    gpu.sync()
+    got, got_lse = out.read(np.float16, q.shape), lse.read(np.float32, (1, n)).T
+    assert np.isfinite(got).all()
+    k, v = cache.rows(0, start + n)
+    for some in ([0, 1, 30], [32760, 32767, 32768], [65534, 65535, 65536, n - 1]):
+        vis = kv8.visible(start + np.asarray(some), start + n, 33, 2)
+        o, l, ds = kv8.attend(q[some], k, v, vis, d ** -0.5)
+        check(got[some], got_lse[some], o, l, ds, v_top(v, vis), int(vis.sum(1).max()), True, f"queries {some}")
