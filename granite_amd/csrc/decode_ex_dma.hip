@@ -18,6 +18,11 @@
 // flight.  No barriers.  What belongs to a tile (pool rows of its two runs of 16 tokens, their scales) is worked out 32
 // tiles at a time, a lane per run; its block-table entries and scales come through LDS as well, since a load the
 // compiler waits for would wait for all transfers in flight.
+//
+// Measured (group of 4 or 8 heads over 8 KV heads of 128, half Q, whole call with the merge): 64 sequences of 256 to 8192 tokens
+// 97 us for 556 MB, 5.7 TB/s; 2 of 131072 92 us for 515 MB, 5.6 TB/s.  Without the arithmetic (timing only) the kernel takes
+// as long: what bounds it is the pattern of memory accesses, 7 us until the first tiles have come and waves that end
+// 15 to 28 us apart.
 #include "common.h"
 #include "kv_attend.h"
 
