@@ -13,9 +13,9 @@
 // against top / 448, x / scale is exact, and growing a scale is exact as well for codes that stay above 2^-6.
 //
 // One launch of up to three kinds of workgroups:
-//   * run of tokens of one sequence: one, two or four waves per (block the run touches, KV head), by the block
+//   * run of tokens of one sequence: one to sixteen waves per (block the run touches, KV head), by the block
 //     size.  They take the block's new rows in turn and keep them in registers between the maximum and the
-//     codes (8 rows of 128 or 16 of 64 elements a wave; what four waves cannot hold is read twice),
+//     codes (8 rows of 128 or 16 of 64 elements a wave; what sixteen waves cannot hold is read twice),
 //   * one token per sequence: a wave per (token, KV head), K in its lower half and V in its upper,
 //   * Q: a thread per eight elements of a token's row in one or kQHeads heads, cos and sin loaded once for all.
 //
@@ -30,7 +30,8 @@
 namespace ghip {
 namespace {
 
-constexpr uint32_t kThreads = 256, kWaves = 4;
+constexpr uint32_t kWaves = 4;      // of a workgroup, but for blocks of so many tokens that four waves do not hold them
+constexpr uint32_t kMaxWaves = 16;
 constexpr int kHold = 2;         // passes of a wave over new rows that stay in registers
 constexpr uint32_t kQHeads = 2;  // heads per thread of the Q part of a large launch
 constexpr float kF8Max = 448.0f;
@@ -165,11 +166,12 @@ __device__ __forceinline__ float wave_max(float v, int from) {
 template <bool kSrcF16, int kD>
 __device__ void append_run(const RopeQ8Params& p) {
     constexpr uint32_t kOcts = kD / 8, kRowsPerPass = 64 / kOcts;
-    __shared__ float s_top[kWaves][2];
+    __shared__ float s_top[kMaxWaves][2];
+    const uint32_t n_waves = blockDim.x / 64;
     const uint32_t lane = threadIdx.x & 63, wave = uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
     const uint32_t part = wave % p.unit_waves;  // of the waves that share a unit
-    const uint32_t unit = min(blockIdx.x * (kWaves / p.unit_waves) + wave / p.unit_waves, p.kv_units - 1);
-    const bool spare = blockIdx.x * (kWaves / p.unit_waves) + wave / p.unit_waves >= p.kv_units;
+    const uint32_t unit = min(blockIdx.x * (n_waves / p.unit_waves) + wave / p.unit_waves, p.kv_units - 1);
+    const bool spare = blockIdx.x * (n_waves / p.unit_waves) + wave / p.unit_waves >= p.kv_units;
     const uint32_t head = unit % p.num_heads_k, blk = p.start_pos / p.block_size + unit / p.num_heads_k;
     const uint32_t end = p.start_pos + p.seq_len;
     const uint32_t lo = max(p.start_pos, blk * p.block_size), hi = min(end, (blk + 1) * p.block_size);  // positions
@@ -319,7 +321,7 @@ template <bool kSrcF16, int kD>
 __device__ void rotate_q(const RopeQ8Params& p) {
     constexpr uint32_t kOcts = kD / 8;
     const uint32_t runs = (p.num_heads_q + p.q_heads - 1) / p.q_heads;
-    const uint64_t idx = uint64_t(blockIdx.x - p.kv_groups) * kThreads + threadIdx.x;
+    const uint64_t idx = uint64_t(blockIdx.x - p.kv_groups) * blockDim.x + threadIdx.x;
     const uint32_t j = uint32_t(idx % kOcts);
     const uint64_t rest = idx / kOcts;
     if (rest >= uint64_t(runs) * p.seq_len) return;
@@ -351,7 +353,7 @@ __device__ void rotate_q(const RopeQ8Params& p) {
 }
 
 template <bool kSrcF16, int kD>
-__global__ void __launch_bounds__(kThreads) rope_q8_kernel(RopeQ8Params p) {
+__global__ void __launch_bounds__(kMaxWaves* kWave) rope_q8_kernel(RopeQ8Params p) {
     if (blockIdx.x >= p.kv_groups) rotate_q<kSrcF16, kD>(p);
     else if (p.positions) append_step<kSrcF16, kD>(p);
     else append_run<kSrcF16, kD>(p);
@@ -418,14 +420,22 @@ int launch_rope_append_q8(const granite_hip_rope_q8_args& a) {
     p.q_out_f32 = a.q_out_dtype == GRANITE_HIP_F32;
 
     uint64_t kv_groups = 0, q_groups = 0;
+    uint32_t n_waves = kWaves;
     if (a.k) {
         const uint64_t units = a.positions ? uint64_t(a.seq_len)
                                            : uint64_t((end - 1) / a.block_size) - a.start_pos / a.block_size + 1;
         if (units * a.num_heads_k > 0x7FFFFFFFull) return GRANITE_HIP_EINVAL;
         p.kv_units = uint32_t(units * a.num_heads_k);
         const uint32_t held = kHold * (512 / a.head_dim);  // rows a wave holds
-        p.unit_waves = a.block_size <= held ? 1 : a.block_size <= 2 * held ? 2 : 4;
-        const uint32_t per_group = a.positions ? kWaves : kWaves / p.unit_waves;
+        p.unit_waves = 1;
+        // as many waves as hold the block's rows, more than four only at head size 128 and while a launch has no more than 4096 of
+        // them: blocks of 128 tokens, 64 units 23.9 us with four waves, 18 with eight, 13.6 with sixteen; 784 units 40, 43 and
+        // 50; at head size 64 16.2 us with four, 18.4 with eight (176 units)
+        const uint32_t most = a.positions || a.head_dim == 64 ? kWaves : kMaxWaves;
+        while (p.unit_waves < most && p.unit_waves * held < a.block_size && (p.unit_waves < kWaves || 2ull * p.unit_waves * p.kv_units <= 4096))
+            p.unit_waves *= 2;
+        if (!a.positions) n_waves = max(kWaves, p.unit_waves);
+        const uint32_t per_group = a.positions ? kWaves : n_waves / p.unit_waves;
         kv_groups = (units * a.num_heads_k + per_group - 1) / per_group;
     }
     if (a.q) {
@@ -434,11 +444,11 @@ int launch_rope_append_q8(const granite_hip_rope_q8_args& a) {
         // (256 CUs x 2048): the lookup of cos and sin is then shared by two heads (8187 tokens: 62.5 us; by four 65)
         p.q_heads = octs >= (2ull << 20) ? kQHeads : 1;
         const uint64_t threads = uint64_t(a.seq_len) * (a.head_dim / 8) * ((a.num_heads_q + p.q_heads - 1) / p.q_heads);
-        q_groups = (threads + kThreads - 1) / kThreads;
+        q_groups = (threads + 64 * n_waves - 1) / (64 * n_waves);
     }
     if (kv_groups + q_groups > 0x7FFFFFFFull) return GRANITE_HIP_EINVAL;
     p.kv_groups = uint32_t(kv_groups);
-    const dim3 grid(uint32_t(kv_groups + q_groups)), block(kThreads);
+    const dim3 grid(uint32_t(kv_groups + q_groups)), block(64 * n_waves);
     hipStream_t st = ctx().stream;
     {
         KernelTimerScope timer("rope_append_q8");
