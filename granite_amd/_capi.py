@@ -7,6 +7,7 @@ raised.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libgranite_hip.so"
@@ -227,13 +228,11 @@ SIGNATURES = {
     "granite_hip_attention_workspace_required": (_int, [C.POINTER(AttentionArgs), C.POINTER(C.c_size_t)]),
     "granite_hip_decode_attention_ws": (_int, [C.POINTER(DecodeArgs), _vp, C.c_size_t]),
     "granite_hip_attention_ws": (_int, [C.POINTER(AttentionArgs), _vp, C.c_size_t]),
-    "granite_hip_decode_attention_ex": (_int, [C.POINTER(DecodeArgs), C.POINTER(KvForm), _vp, C.c_size_t]),
-    "granite_hip_attention_ex": (_int, [C.POINTER(AttentionArgs), C.POINTER(KvForm), _vp, C.c_size_t]),
-    "granite_hip_decode_ex_workspace_required": (
-        _int, [C.POINTER(DecodeArgs), C.POINTER(KvForm), C.POINTER(C.c_size_t)]),
-    "granite_hip_attention_ex_workspace_required": (
-        _int, [C.POINTER(AttentionArgs), C.POINTER(KvForm), C.POINTER(C.c_size_t)]),
-    "granite_hip_rope_append_q8": (_int, [C.POINTER(RopeQ8Args)]),
+    "granite_hip_decode_attention_ex": (_int, [_vp, _vp, _vp, C.c_size_t]),  # (bytes of packed(), or byref of the structures)
+    "granite_hip_attention_ex": (_int, [_vp, _vp, _vp, C.c_size_t]),
+    "granite_hip_decode_ex_workspace_required": (_int, [_vp, _vp, C.POINTER(C.c_size_t)]),
+    "granite_hip_attention_ex_workspace_required": (_int, [_vp, _vp, C.POINTER(C.c_size_t)]),
+    "granite_hip_rope_append_q8": (_int, [_vp]),
     "granite_hip_decode_attention_static": (_int, [C.POINTER(DecodeArgs)]),
     "granite_hip_static_scratch_bytes": (C.c_size_t, []),
 }
@@ -258,6 +257,22 @@ def load() -> C.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def packed(cls):
+    """A function that lays out a value per field as the bytes of the ctypes structure `cls`, pointers being ints:
+    a third of the time of filling the structure, which counts where a launch takes a few microseconds."""
+    codes = {C.c_void_p: "P", C.c_int: "i", C.c_uint32: "I", C.c_int64: "q", C.c_float: "f"}
+    layout = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0P")
+    assert layout.size == C.sizeof(cls)
+    pack = layout.pack
+
+    def block(*values) -> bytes:
+        try:
+            return pack(*values)
+        except struct.error:  # out of a field's range: as ctypes takes it
+            return bytes(cls(*values))
+    return block
 
 
 def check(code: int, what: str) -> None:

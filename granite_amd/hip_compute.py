@@ -15,7 +15,7 @@ import numpy as np
 from . import _capi
 from ._capi import (F16, F32, F8E4M3, MASK_CAUSAL, MASK_NONE, MASK_TREE, MEM_DEVICE, ROUND_NEAREST,
                     ROUND_TRUNCATE, AttentionArgs, KvForm, RopeArgs, RopeQ8Args,
-                    DecodeArgs, check)
+                    DecodeArgs, check, packed)
 
 
 class DeviceBuffer:
@@ -73,8 +73,11 @@ def _p(buf) -> Optional[int]:
 
 
 def _ptrs(*bufs) -> list:
-    """_p of each: one call where a launch of a few microseconds has a dozen pointers."""
-    return [b if b is None or type(b) is int else _p(b) for b in bufs]
+    """_p of each, None as 0: one call where a launch of a few microseconds has a dozen pointers."""
+    return [b if type(b) is int else 0 if b is None else _p(b) for b in bufs]
+
+
+_decode_args, _attention_args, _kv_form, _rope_q8_args = map(packed, (DecodeArgs, AttentionArgs, KvForm, RopeQ8Args))
 
 
 class HipCompute:
@@ -289,17 +292,17 @@ class HipCompute:
         first num_sinks."""
         q, k_cache, v_cache, block_tables, seq_lens, out, lse, k_scale, v_scale = _ptrs(
             q, k_cache, v_cache, block_tables, seq_lens, out, lse, k_scale, v_scale)
-        a = DecodeArgs(q, q_dtype, k_cache, v_cache, block_tables, seq_lens, out, lse, batch_size,
-                       num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, max_seq, scale,
-                       fixed_seq_len, 0)
-        f = KvForm(kv_dtype, k_scale, v_scale, num_blocks, window, num_sinks)
+        a = _decode_args(q, q_dtype, k_cache, v_cache, block_tables, seq_lens, out, lse, batch_size,
+                         num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, max_seq, scale,
+                         fixed_seq_len, 0)
+        f = _kv_form(kv_dtype, k_scale, v_scale, num_blocks, window, num_sinks)
         if query_workspace:
             need = C.c_size_t()
-            check(self.lib.granite_hip_decode_ex_workspace_required(C.byref(a), C.byref(f), C.byref(need)),
+            check(self.lib.granite_hip_decode_ex_workspace_required(a, f, C.byref(need)),
                   "decode_ex_workspace_required")
             return need.value
         ws, ws_bytes = self._workspace(workspace, workspace_bytes)
-        check(self.lib.granite_hip_decode_attention_ex(C.byref(a), C.byref(f), ws, ws_bytes), "decode_attention_ex")
+        check(self.lib.granite_hip_decode_attention_ex(a, f, ws, ws_bytes), "decode_attention_ex")
 
     def attention_ex(self, *, q, q_dtype, q_tok_stride, q_head_stride, out, out_dtype, out_tok_stride,
                      out_head_stride, seq_q, num_heads, num_kv_heads, head_dim, scale, k_cache, v_cache, cache_len,
@@ -310,17 +313,17 @@ class HipCompute:
         position start_pos + index."""
         q, out, lse, k_cache, v_cache, block_table, k_scale, v_scale = _ptrs(
             q, out, lse, k_cache, v_cache, block_table, k_scale, v_scale)
-        a = AttentionArgs(q, q_dtype, q_tok_stride, q_head_stride, out, out_dtype, out_tok_stride, out_head_stride,
-                          lse, k_cache, v_cache, block_table, block_size, max_seq, cache_len, None, None, 0, None, mask_mode, start_pos, seq_q, num_heads, num_kv_heads,
-                          head_dim, scale)
-        f = KvForm(kv_dtype, k_scale, v_scale, num_blocks, window, num_sinks)
+        a = _attention_args(q, q_dtype, q_tok_stride, q_head_stride, out, out_dtype, out_tok_stride, out_head_stride,
+                            lse, k_cache, v_cache, block_table, block_size, max_seq, cache_len, 0, 0, 0, 0, mask_mode,
+                            start_pos, seq_q, num_heads, num_kv_heads, head_dim, scale)
+        f = _kv_form(kv_dtype, k_scale, v_scale, num_blocks, window, num_sinks)
         if query_workspace:
             need = C.c_size_t()
-            check(self.lib.granite_hip_attention_ex_workspace_required(C.byref(a), C.byref(f), C.byref(need)),
+            check(self.lib.granite_hip_attention_ex_workspace_required(a, f, C.byref(need)),
                   "attention_ex_workspace_required")
             return need.value
         ws, ws_bytes = self._workspace(workspace, workspace_bytes)
-        check(self.lib.granite_hip_attention_ex(C.byref(a), C.byref(f), ws, ws_bytes), "attention_ex")
+        check(self.lib.granite_hip_attention_ex(a, f, ws, ws_bytes), "attention_ex")
 
     def rope_append_q8(self, *, seq_len, head_dim, src_dtype, q=None, q_out=None, q_out_dtype=F16, num_heads_q=0,
                        k=None, v=None, num_heads_k=0, k_cache=None, v_cache=None, k_scale=None, v_scale=None,
@@ -331,10 +334,10 @@ class HipCompute:
         (rotated) and V appended as e4m3 codes."""
         q, q_out, k, v, k_cache, v_cache, k_scale, v_scale, block_table, cos_table, sin_table, positions = _ptrs(
             q, q_out, k, v, k_cache, v_cache, k_scale, v_scale, block_table, cos_table, sin_table, positions)
-        a = RopeQ8Args(q, q_out, k, v, src_dtype, q_out_dtype, k_cache, v_cache, k_scale, v_scale, block_table,
-                       cos_table, sin_table, table_positions, freq_base, num_heads_q, num_heads_k, seq_len,
-                       head_dim, start_pos, block_size, num_blocks, max_blocks_per_seq, positions, table_stride)
-        check(self.lib.granite_hip_rope_append_q8(C.byref(a)), "rope_append_q8")
+        check(self.lib.granite_hip_rope_append_q8(_rope_q8_args(
+            q, q_out, k, v, src_dtype, q_out_dtype, k_cache, v_cache, k_scale, v_scale, block_table,
+            cos_table, sin_table, table_positions, freq_base, num_heads_q, num_heads_k, seq_len,
+            head_dim, start_pos, block_size, num_blocks, max_blocks_per_seq, positions, table_stride)), "rope_append_q8")
 
     # ---- scratch memory
     def workspace_bytes(self) -> int:

@@ -144,3 +144,14 @@ def test_new_structures_match_the_header():
         body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
         fields = [part.strip().split()[-1].lstrip("*") for d in body.split(";") if d.strip() for part in d.strip().split(",")]
         assert fields == [f[0] for f in cls._fields_], cname
+
+
+@pytest.mark.parametrize("cls", [_capi.DecodeArgs, _capi.AttentionArgs, _capi.KvForm, _capi.RopeQ8Args])
+def test_packed_arguments_are_the_structures(cls):
+    """HipCompute hands these structures over as bytes."""
+    block = _capi.packed(cls)
+    plain = [(0.5 if t is C.c_float else 3 * i + 1) for i, (_, t) in enumerate(cls._fields_)]
+    odd = [(-2.5 if t is C.c_float else -1) for _, t in cls._fields_]  # wraps where a field has no sign
+    for values in (plain, odd):
+        got, want = cls.from_buffer_copy(block(*values)), cls(*values)
+        assert [getattr(got, n) for n, _ in cls._fields_] == [getattr(want, n) for n, _ in cls._fields_]
