@@ -4,9 +4,9 @@ import numpy as np
 import pytest
 
 import kv8
-from granite_amd import F16, F32, F8E4M3
+from granite_amd import F16, F32, F8E4M3, MASK_CAUSAL
 from gpu_util import dev, say
-from test_gpu_kv_ex import NAN8, Cache, check, v_top
+from test_gpu_kv_ex import NAN8, Cache, Captured, check, v_top
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,47 @@ def test_nan_and_infinities(gpu):
     half.k[at(half, 4, 101), 1, 7] = np.inf
     got, _ = run(gpu, half.upload(), 16, F16, 2500, 4, some=(2, 3, 4, 5))
     assert np.isposinf(got[3, 1, 7]) and np.isnan(got[3, 2, 7]) and (~np.isfinite(got)).sum() == 2
+
+
+def test_captured_launches_of_every_kernel(gpu):
+    """The persistent kernels with their merges, and the tiles kernel with keys cut, each in a graph with a workspace of its
+    own: replays with other queries and lengths, in turn and with eager calls between them, equal the eager calls."""
+    rng = np.random.default_rng(30)
+    graphs, jobs = [], []
+    for kv, hq, hkv, d, window in ((F8E4M3, 16, 16, 64, 0), (F16, 24, 24, 64, 2600)):
+        cache = Cache(rng, [2900] * 24, 48, hkv, d, kv).upload()
+        q, out, lse, n = (dev(np.zeros((24, hq, d), np.float16)), dev(np.zeros((24, hq, d), np.float32)), dev(np.zeros((24, hq), np.float32)),
+                          dev(np.full(24, 2900, np.int32)))
+        kw = dict(q=q, q_dtype=F16, out=out, lse=lse, batch_size=24, num_heads=hq, scale=0.1, block_tables=cache.dev[4], seq_lens=n,
+                  max_blocks_per_seq=cache.max_blocks, window=window, num_sinks=3, **cache.kwargs())
+        jobs.append((gpu.decode_attention_ex, kw, q, out, lse, n, cache))
+    cache = Cache(rng, [4000], 20, 2, 64, F8E4M3).upload()
+    q, out, lse = dev(np.zeros((300, 96, 64), np.float16)), dev(np.zeros((300, 96, 64), np.float16)), dev(np.zeros((96, 300), np.float32))
+    kw = dict(q=q, q_dtype=F16, q_tok_stride=96 * 64, q_head_stride=64, out=out, out_dtype=F16, out_tok_stride=96 * 64, out_head_stride=64,
+              seq_q=300, num_heads=96, scale=0.1, cache_len=4000, block_table=cache.dev[4], mask_mode=MASK_CAUSAL, start_pos=3700, lse=lse,
+              **cache.kwargs())
+    jobs.append((gpu.attention_ex, kw, q, out, lse, None, cache))
+    for call, kw, q, out, lse, n, _ in jobs:
+        need = call(**kw, query_workspace=True)
+        assert need > 0
+        kw["workspace"] = dev(np.zeros(need, np.uint8))
+        graphs.append(Captured(gpu, lambda call=call, kw=kw: call(**kw)))
+    for i in range(4):
+        for _, _, q, out, lse, n, _ in jobs:
+            q.write(rng.standard_normal(q.nbytes // 2).astype(np.float16))
+            out.fill(0)
+            lse.fill(0)
+            if n is not None:
+                n.write(rng.integers(1, 2901, 24).astype(np.int32))
+        for g in graphs:
+            g.replay()
+        replayed = [(out.read(np.uint8, out.nbytes), lse.read(np.uint8, lse.nbytes)) for _, _, _, out, lse, _, _ in jobs]
+        for (call, kw, _, out, lse, _, _), got in zip(jobs, replayed):
+            out.fill(0)
+            lse.fill(0)
+            call(**kw)
+            gpu.sync()
+            assert np.array_equal(got[0], out.read(np.uint8, out.nbytes)) and np.array_equal(got[1], lse.read(np.uint8, lse.nbytes)), f"replay {i}"
+            assert got[0].any()
+    for g in graphs:
+        g.close()
