@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         const uint32_t it = min(t_begin + kPlan * block + lane, n_tiles - 1);
         return min(seen.tile(it) * kBN + wave_key + 4 * f, (seen.end - 1) & (kFine ? ~3u : ~7u));
     };
-    // step 1: the block-table entries
+    // the block-table entries
     struct Entries {
         int32_t e[kPieceRuns];
     };
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         for (int f = 0; f < kPieceRuns; f++) r.e[f] = kRows == kExContiguous ? 0 : p.tables[plan_key(block, f) / p.block_size];
         return r;
     };
-    // step 2: pool row of the first key, bit 31: the page is one of the pool's; and the scales of its run
+    // pool row of the first key, bit 31: the page is one of the pool's; and the scales of its run
     struct Plan {
         uint32_t row[kPieceRuns];
         float ks[kPieceRuns], vs[kPieceRuns];
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         }
         return r;
     };
-    // step 3: what the softmax takes from the scales, for every wave.  A run that nobody sees may have anything for
+    // what the softmax takes from the scales, for every wave.  A run that nobody sees may have anything for
     // scales; a masked score, minus infinity, must come through the factor and the shift as what it is: a positive
     // factor, a finite shift.
     auto plan_runs = [&](const Plan& r, uint32_t half) __attribute__((always_inline)) {
@@ -552,7 +552,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         // the second and third, and the rows of the first 64
         Piece a, b;
         Plan cur = plan_rows(0, plan_entries(0));
-        Entries next_entries = {};
         Plan next = cur;
         auto row_of = [&](uint32_t j) __attribute__((always_inline)) -> At {
             At at;
@@ -607,12 +606,14 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
                 at_v2 = at_v;
                 at_v = at_k;
             }
-            if (part == 5) {  // the next 64 tiles, in three steps a few tiles apart
+            if (part == 5) {
+                // the next 64 tiles.  In one go, with two waits for memory: what three steps a few tiles apart would carry from
+                // one to the next costs more in registers (512 at 32768: 541 us, so 534; with float queries and results over
+                // blocks of 8 tokens, 24407 keys, 1353 and 1148)
                 const uint32_t j = it + 4 - t_begin, block = j / kPlan + 1;
-                if (t_begin + block * kPlan < n_tiles) {
-                    if (j % kPlan == 32) next_entries = plan_entries(block);
-                    else if (j % kPlan == 40) next = plan_rows(block, next_entries);
-                    else if (j % kPlan == 48) plan_runs(next, block & 1);
+                if (j % kPlan == 40 && t_begin + block * kPlan < n_tiles) {
+                    next = plan_rows(block, plan_entries(block));
+                    plan_runs(next, block & 1);
                 }
             }
         };
