@@ -128,12 +128,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     const uint32_t all_hi = limit_of(wg_first), all_lo = window_begin(wg_last, p.window);  // seen by every row
     const uint32_t t_begin = uint32_t(uint64_t(seen.count) * split / p.n_splits);
     const uint32_t n_tiles = uint32_t(uint64_t(seen.count) * (split + 1) / p.n_splits);
-    // keys from `cap` on belong to the next split: the tile that a wave may compute beyond its share is masked whole
-    const uint32_t cap = n_tiles < seen.count ? seen.tile(n_tiles) * kBN : 0xFFFFFFFFu;
     const uint32_t wave_first = pos_of(r0), wave_last = pos_of(r0 + 31);
     const uint32_t wave_hi = limit_of(wave_last);  // behind the last key any row of the wave sees
-    const uint32_t every_hi = min(limit_of(wave_first), cap), every_lo = window_begin(wave_last, p.window);  // every row sees
-    const uint32_t row_hi = min(limit_of(p.start_pos + query), cap), row_lo = window_begin(p.start_pos + query, p.window);
+    const uint32_t every_hi = limit_of(wave_first), every_lo = window_begin(wave_last, p.window);  // every row sees
+    const uint32_t row_hi = limit_of(p.start_pos + query), row_lo = window_begin(p.start_pos + query, p.window);
 
     // ---- Q^T as B operand: lane (n, g), step s holds Q[row][16 s + 8 g .. + 7]
     half8 bq[kSteps];
@@ -536,8 +534,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     if (tid == 0) *s_special = 0;
     __syncthreads();
     if (t_begin < n_tiles) {  // uniform; an empty share writes a neutral partial
-        // Tiles this wave computes: up to the last one that holds a key some row of it sees, in pairs (a tile that
-        // is one too many, or in front of a later window's first, is masked whole).  There is one code path: both
+        // Tiles this wave computes: up to the last one that holds a key some row of it sees (one in front of a later
+        // window's first is masked whole).  There is one code path: both
         // phases run in every iteration, and where a stage does not apply yet it works on zero probabilities.
         uint32_t my_end = t_begin;
         if (wave_active)
@@ -546,11 +544,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
                     my_end = it;
                     break;
                 }
-        my_end += (my_end - t_begin) & 1;
 
-        // ---- prologue: in LDS K of the first two tiles and V of the first, in flight K of the third and fourth and V of
-        // the second and third, and the rows of the first 64
-        Piece a, b;
+        // ---- prologue: in LDS K of the first two tiles and V of the first, in flight K of the third and V of the second, and
+        // the rows of the first 64.  An iteration is long enough for what is loaded in one to be there in the next (a second
+        // piece in flight gained nothing and cost registers: 935 us for 512 queries with float results at 32768, 895 without).
+        Piece a;
         Plan cur = plan_rows(0, plan_entries(0));
         Plan next = cur;
         auto row_of = [&](uint32_t j) __attribute__((always_inline)) -> At {
@@ -559,24 +557,23 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             for (int f = 0; f < kPieceRuns; f++) at.row[f] = uint32_t(__builtin_amdgcn_readlane(int(cur.row[f]), int(j % kPlan)));
             return at;
         };
-        const At o0 = row_of(0), o1 = row_of(1), o2 = row_of(2), o3 = row_of(3);
-        load_k(o0, a);
-        load_v(o0, a);
-        load_k(o1, b);
-        plan_runs(cur, 0);
-        plan_runs(cur, 1);  // (tiles behind the last, which are masked, find valid numbers)
-        store_k(0, a);
-        store_v(0, t_begin, o0, a);
-        store_k(1, b);
+        const At o0 = row_of(0), o1 = row_of(1), o2 = row_of(2);
+        {
+            Piece b;
+            load_k(o0, a);
+            load_v(o0, a);
+            load_k(o1, b);
+            plan_runs(cur, 0);
+            plan_runs(cur, 1);  // (tiles behind the last, whose scores nobody takes, find numbers)
+            store_k(0, a);
+            store_v(0, t_begin, o0, a);
+            store_k(1, b);
+        }
         __builtin_amdgcn_sched_barrier(0);
         load_k(o2, a);
         load_v(o1, a);
         __builtin_amdgcn_sched_barrier(0);
-        load_k(o3, b);
-        load_v(o2, b);
-        __builtin_amdgcn_sched_barrier(0);
-        At at_v = o3;                // of the tile whose V is loaded next
-        At at_v1 = o1, at_v2 = o2;  // of those whose V is in flight: stored next, and the one after
+        At at_v = o2, at_v1 = o1;  // of the tile whose V is loaded next, and of the one whose V is in flight
         __syncthreads();
 
         float16v s0, s1;
@@ -593,24 +590,23 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         uint32_t kb_cur = 0, kb_next = 1, kb_store = 2;
         // (the first iteration's second product, of nothing, reads the first tile's V: whatever it holds, every row sees it)
         uint32_t vb_prev = 0, vb_cur = 0, vb_store = 1;
-        auto staging = [&](uint32_t it, Piece& piece, int part) __attribute__((always_inline)) {
-            if (part == 0) store_k(kb_store, piece);                  // K of tile it + 2
-            if (part == 2) store_v(vb_store, it + 1, at_v1, piece);  // V of tile it + 1
-            if (part == 4) {  // K of it + 4, V of it + 3
-                const uint32_t j = it + 4 - t_begin;
+        auto staging = [&](uint32_t it, int part) __attribute__((always_inline)) {
+            if (part == 0) store_k(kb_store, a);                  // K of tile it + 2
+            if (part == 2) store_v(vb_store, it + 1, at_v1, a);  // V of tile it + 1
+            if (part == 4) {  // K of it + 3, V of it + 2
+                const uint32_t j = it + 3 - t_begin;
                 if (j % kPlan == 0) cur = next;
                 const At at_k = row_of(j);
-                load_k(at_k, piece);
-                load_v(at_v, piece);
-                at_v1 = at_v2;
-                at_v2 = at_v;
+                load_k(at_k, a);
+                load_v(at_v, a);
+                at_v1 = at_v;
                 at_v = at_k;
             }
             if (part == 5) {
                 // the next 64 tiles.  In one go, with two waits for memory: what three steps a few tiles apart would carry from
                 // one to the next costs more in registers (512 at 32768: 541 us, so 534; with float queries and results over
                 // blocks of 8 tokens, 24407 keys, 1353 and 1148)
-                const uint32_t j = it + 4 - t_begin, block = j / kPlan + 1;
+                const uint32_t j = it + 3 - t_begin, block = j / kPlan + 1;
                 if (j % kPlan == 40 && t_begin + block * kPlan < n_tiles) {
                     next = plan_rows(block, plan_entries(block));
                     plan_runs(next, block & 1);
@@ -630,35 +626,29 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         // At head size 64 a phase has too few MFMAs to cover all of the staging: it is spread over both (196 us against
         // 204 for 4096 queries with a window of 4096; at 128 the second phase covers nothing more: 550 against 538 for 512 at 32768).
         constexpr bool kSpread = kD == 64;
-        auto iteration = [&](uint32_t it, Piece& piece) __attribute__((always_inline)) {
+        auto iteration = [&](uint32_t it) __attribute__((always_inline)) {
             const uint32_t key_cur = key_of(it), key_nxt = key_of(it + 1);
             const Runs ra = runs_of(it, 0);
             fused_phase(it, key_cur + 32, kb_cur, 1, s1, s0, ra, p_new, vb_prev, 1, p_old, [&](int step) {
                 const int part = step - (kPhase - 8);
-                if (!kSpread || part == 0) staging(it, piece, part);
+                if (!kSpread || part == 0) staging(it, part);
             });
             const Runs rb = runs_of(it, 1);
             fused_phase(it + 1, key_nxt, kb_next, 0, s0, s1, rb, p_old, vb_cur, 0, p_new, [&](int step) {
                 const int part = step - (kPhase - 8) + 2;
-                if (kSpread && part >= 2) staging(it, piece, part);
+                if (kSpread && part >= 2) staging(it, part);
             });
             rotate_buffers();
         };
-        auto stage_only = [&](uint32_t it, Piece& piece) __attribute__((always_inline)) {
+        auto stage_only = [&](uint32_t it) __attribute__((always_inline)) {
 #pragma unroll
-            for (int part = 0; part < 6; part++) staging(it, piece, part);
+            for (int part = 0; part < 6; part++) staging(it, part);
             rotate_buffers();
         };
         uint32_t it = t_begin;
-        for (; it < my_end; it += 2) {
-            iteration(it, a);
-            iteration(it + 1, b);
-        }
+        for (; it < my_end; it++) iteration(it);
         if (my_end > t_begin) accumulate(vb_prev, 1, p_old);
-        for (; it < n_tiles; it += 2) {
-            stage_only(it, a);
-            stage_only(it + 1, b);
-        }
+        for (; it < n_tiles; it++) stage_only(it);
     }
 
     if (!wave_active) return;
