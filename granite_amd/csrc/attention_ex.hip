@@ -22,8 +22,8 @@
 //   two subtractions and one more multiply-add than without scales.
 // * Tiles are visited by the list of kv_visible.h: those of the sinks, then those of the window.
 //
-// Measured (half Q and results): 512 queries of 64 heads over 8 KV heads of 128 behind 32768 keys 562 us a call, 0.99 PFLOP/s
-// (a large half matrix product reaches 1.17); 4096 queries of 32 heads of 64 through a window of 4096 203 us, 0.68 PFLOP/s;
+// Measured (half Q and results): 512 queries of 64 heads over 8 KV heads of 128 behind 32768 keys 535 to 572 us a call, 1.0 PFLOP/s
+// (a large half matrix product reaches 1.17); 4096 queries of 32 heads of 64 through a window of 4096 198 us, 0.69 PFLOP/s;
 // 2048 queries of 32 heads of 128 through a window of 512 31 us.  What bounds it: a tile is 64 MFMAs on a SIMD, 2048 cycles,
 // and some 370 vector instructions beside them (softmax, conversions of codes and probabilities), 6 a MFMA at head size
 // 128 and 11 at 64; the matrix cores are busy 45 % (27 %) of the time.

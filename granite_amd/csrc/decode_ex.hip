@@ -3,7 +3,7 @@
 //
 // The row kernel takes 16 rows of a KV head a workgroup; its eight waves take the visible tiles (64 tokens of 8 bits, 32 of half) in
 // turn, straight from memory as MFMA operands, and are joined through LDS, so a call is one launch unless its keys are
-// cut.  One sequence of 512 tokens 8.3 us a call (a wave has one tile; launch and first loads), 64 sequences of
+// cut.  One sequence of 512 tokens 7.9 us a call (a wave has one tile; launch and first loads), 64 sequences of
 // 8192 over blocks of 20 tokens 226 us, 4.8 TB/s.
 #include <cmath>
 

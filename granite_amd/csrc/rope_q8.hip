@@ -19,9 +19,9 @@
 //   * one token per sequence: a wave per (token, KV head), K in its lower half and V in its upper,
 //   * Q: a thread per eight elements of a token's row in one or kQHeads heads, cos and sin loaded once for all.
 //
-// Measured (32 query heads over 8 KV heads of 128): 8187 tokens, half in and float Q out, 59.6 us a call for 256 MB, 4.3 TB/s,
+// Measured (32 query heads over 8 KV heads of 128): 8187 tokens, half in and float Q out, 59.9 us a call for 256 MB, 4.3 TB/s,
 // where a large copy reaches 4.9 (66 us with one head a thread and a wave a block); 64 tokens of 64 sequences 3.2 us of
-// kernel in a call of 8.3 us: the launch; 512 tokens (64 heads) 8.4 us a call, 3.7 TB/s.
+// kernel in a call of 7.8 us: the launch; 512 tokens (64 heads) 8.4 us a call, 3.7 TB/s.
 #include <cmath>
 
 #include "common.h"
