@@ -506,7 +506,8 @@ int granite_hip_decode_attention_ex(const granite_hip_decode_args *args,
 int granite_hip_attention_ex(const granite_hip_attention_args *args,
                              const granite_hip_kv_form *form, void *workspace,
                              size_t workspace_bytes);
-/* Scratch bytes the launch needs, as granite_hip_decode_workspace_required. */
+/* Scratch bytes the launch needs, as granite_hip_decode_workspace_required.  They are those of a launch of exactly these
+ * sizes: how keys are cut depends on them, and a smaller launch may need more than a larger one. */
 int granite_hip_decode_ex_workspace_required(const granite_hip_decode_args *args,
                                              const granite_hip_kv_form *form, size_t *bytes);
 int granite_hip_attention_ex_workspace_required(const granite_hip_attention_args *args,
