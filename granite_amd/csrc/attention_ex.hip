@@ -834,7 +834,6 @@ int launch_kv_tiles(KvParams p, const KvCall& call, bool q_f32, int rows, const 
     const uint32_t D = call.head_dim;
     const bool f8 = call.f8;
     const uint64_t n_rows = uint64_t(p.seq_q) * p.group;
-    if (n_rows >= (1ull << 31)) return GRANITE_HIP_EINVAL;
     p.q_tiles = uint32_t((n_rows + kBM - 1) / kBM);
     // With a window every row sees about as many keys, and behind a long prefix nearly as many.
     p.paired = p.causal && p.window == 0 && p.start_pos < 4 * uint64_t(p.seq_q);

@@ -322,6 +322,7 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     if (a.mask_mode == GRANITE_HIP_MASK_NONE && f.window != 0) return GRANITE_HIP_EUNSUPPORTED;
     if (a.cache_len == 0 || a.cache_len >= (1u << 31)) return GRANITE_HIP_EINVAL;
     if (uint64_t(a.start_pos) + a.seq_q >= (1ull << 31)) return GRANITE_HIP_EINVAL;
+    if (uint64_t(a.seq_q) * (a.num_heads / a.num_kv_heads) >= (1ull << 31)) return GRANITE_HIP_EINVAL;  // rows of a KV head
     if (!a.k_cache || !a.v_cache) return GRANITE_HIP_ENULL;
     if (!a.block_table && a.max_seq < a.cache_len) return GRANITE_HIP_EINVAL;
     const int64_t qes = a.q_dtype == GRANITE_HIP_F32 ? 4 : 2, oes = a.out_dtype == GRANITE_HIP_F32 ? 4 : 2;
@@ -366,7 +367,7 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     const KvCall call = call_of(p, D, q_f32, f8, rows);
     int tile_rows = rows;
     if (rows == kExPagedAny && a.block_size % 4 == 0 && p.row_bytes < (1 << 27)) tile_rows = kExPaged4;
-    const bool tiled = tile_rows != kExPagedAny && call.rows < (1ull << 31);
+    const bool tiled = tile_rows != kExPagedAny;
     const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
     const uint32_t tiles = uint32_t((seen + 31) / 32);
     p.q_groups = uint32_t((call.rows + 15) / 16);

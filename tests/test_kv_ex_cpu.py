@@ -155,3 +155,8 @@ def test_packed_arguments_are_the_structures(cls):
     for values in (plain, odd):
         got, want = cls.from_buffer_copy(block(*values)), cls(*values)
         assert [getattr(got, n) for n, _ in cls._fields_] == [getattr(want, n) for n, _ in cls._fields_]
+
+
+def test_more_rows_than_an_index_holds_are_refused():
+    assert prefill(seq_q=1 << 30, num_heads=8, num_kv_heads=2) == EINVAL
+    assert prefill(seq_q=0, num_heads=8, num_kv_heads=2) in (ENOTINIT, OK)
