@@ -211,12 +211,13 @@ __global__ void __launch_bounds__(kD* kJoin) kv_stream_merge_kernel(KvParams p) 
     const uint32_t b = blockIdx.y, d = threadIdx.x % kD, part = threadIdx.x / kD;
     const uint32_t* prefix = p.plan + kPlanHeader;
     const uint32_t nt = prefix[b + 1] - prefix[b];
-    if (nt == 0) return;  // empty sequence: its output stays
+    if (nt == 0 && p.decode) return;  // empty sequence: its output stays
+    // (several queries whose windows lie behind the cache have no tile either: they see nothing, which is a result)
     const uint32_t per = p.plan[0], per_list = p.plan[1];
     const uint32_t lists = p.num_kv_heads * p.q_groups / per_list;
     const uint32_t vh = kvh * p.q_groups + row / 16, lh = vh / per_list;
     const uint32_t u_start = prefix[b] * lists + lh * nt;
-    const uint32_t first_worker = u_start / per, n_parts = (u_start + nt - 1) / per - first_worker + 1;
+    const uint32_t first_worker = u_start / per, n_parts = nt == 0 ? 0 : (u_start + nt - 1) / per - first_worker + 1;
     const size_t at0 = size_t(first_worker + b * lists + lh) * p.part_cap + (vh % per_list) * (p.part_cap / per_list) + row % 16;
     float mx = kExNegBig, o = 0.0f, l = 0.0f;
     for (uint32_t c0 = 4 * part; c0 < n_parts; c0 += 4 * kJoin) {  // four at a time: their loads are in flight together
