@@ -5,6 +5,7 @@
 // turn, straight from memory as MFMA operands, and are joined through LDS, so a call is one launch unless its keys are
 // cut.  One sequence of 512 tokens 7.9 us a call (a wave has one tile; launch and first loads), 64 sequences of
 // 8192 over blocks of 20 tokens 226 us, 4.8 TB/s.
+#include <algorithm>
 #include <cmath>
 
 #include "common.h"
@@ -167,7 +168,7 @@ KvCall call_of(const KvParams& p, uint32_t D, bool q_f32, bool f8, int rows) {
     c.group = p.group;
     c.head_dim = D;
     c.start_pos = p.start_pos;
-    c.length = p.causal && !p.decode ? uint32_t(min(uint64_t(p.max_tokens), uint64_t(p.start_pos) + p.seq_q)) : p.max_tokens;
+    c.length = p.causal && !p.decode ? uint32_t(std::min(uint64_t(p.max_tokens), uint64_t(p.start_pos) + p.seq_q)) : p.max_tokens;
     c.window_keys = p.window ? uint64_t(p.window) + p.sinks : 0;
     c.causal = p.causal && !p.decode;
     c.f8 = f8;
@@ -238,7 +239,7 @@ int check_form(const granite_hip_kv_form& f, const void* k, const void* v, const
     p.block_size = table ? block_size : 1;
     p.bs_shift = (p.block_size & (p.block_size - 1)) == 0 ? __builtin_ctz(p.block_size) : -1;
     p.window = f.window;
-    p.sinks = f.window ? min(f.num_sinks, 0x7FFFFFFFu) : 0;
+    p.sinks = f.window ? std::min(f.num_sinks, 0x7FFFFFFFu) : 0;  // (std: the unqualified min of host code is one of ints)
     return GRANITE_HIP_OK;
 }
 
@@ -301,7 +302,7 @@ int launch_decode_ex(const granite_hip_decode_args& a, const granite_hip_kv_form
     // Tiles of the longest sequence: its whole length, or its window and sinks and the tiles their ends lie in.
     const bool f8 = f.kv_dtype == GRANITE_HIP_F8E4M3;
     constexpr uint32_t tile = 32;
-    const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + 2 * tile) : p.max_tokens;
+    const uint64_t seen = p.window ? std::min(uint64_t(p.max_tokens), uint64_t(p.window) + p.sinks + 2 * tile) : p.max_tokens;
     const uint32_t tiles = uint32_t((seen + tile - 1) / tile);
     const bool q_f32 = a.q_dtype == GRANITE_HIP_F32;
     const KvCall call = call_of(p, D, q_f32, f8, rows);
@@ -368,12 +369,12 @@ int launch_attention_ex(const granite_hip_attention_args& a, const granite_hip_k
     int tile_rows = rows;
     if (rows == kExPagedAny && a.block_size % 4 == 0 && p.row_bytes < (1 << 27)) tile_rows = kExPaged4;
     const bool tiled = tile_rows != kExPagedAny;
-    const uint64_t seen = p.window ? min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
+    const uint64_t seen = p.window ? std::min(uint64_t(p.max_tokens), uint64_t(p.window) + a.seq_q + p.sinks + 64) : p.max_tokens;
     const uint32_t tiles = uint32_t((seen + 31) / 32);
     p.q_groups = uint32_t((call.rows + 15) / 16);
     const bool streamed = f8 && call.rows <= kStreamRows && kv_stream_supports(p, f8, rows, tiles);
     const double rows_us = kv_rows_cut(call).us, tiles_us = tiled ? kv_tiles_cut(call).us : INFINITY, stream_us = streamed ? kv_stream_us(call) : INFINITY;
-    if (stream_us < min(rows_us, tiles_us)) return launch_kv_stream(p, D, q_f32, f8, rows, tiles, scratch);
+    if (stream_us < std::min(rows_us, tiles_us)) return launch_kv_stream(p, D, q_f32, f8, rows, tiles, scratch);
     if (tiles_us < rows_us) return launch_kv_tiles(p, call, q_f32, tile_rows, scratch);
     return launch_rows(p, D, q_f32, f8, rows, scratch);
 }

@@ -20,6 +20,8 @@
 // block-table entries are a tile further ahead.  Measured (32 heads over 8 KV heads of 128): 64 sequences of 256 to 8192 tokens
 // through a window of 1024 58 us a call for 260 MB, 4.5 TB/s; through one of 4096 170 us, 4.8 TB/s.  All loads are unconditional: a load inside a branch would make the
 // compiler wait for every outstanding one at the join.
+#include <algorithm>
+
 #include "common.h"
 #include "kv_attend.h"
 
@@ -299,8 +301,8 @@ int launch_part(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t 
     const uint32_t lists = vheads / per_list;
     p.workers = cus * (kWaves / per_list);
     // smallest range of a worker: a short batch is not cut into ranges of a tile or two, each with a partial to join
-    p.min_per = max(1u, min(4u, (tiles_per_seq + 31) / 32));
-    p.part_cap = per_list * min(p.seq_q * p.group, 16u);
+    p.min_per = std::clamp((tiles_per_seq + 31) / 32, 1u, 4u);
+    p.part_cap = per_list * std::min(p.seq_q * p.group, 16u);
     const size_t slots = (size_t(p.workers) + size_t(p.batch) * lists) * p.part_cap;
     const size_t plan_bytes = ((kPlanHeader + size_t(p.batch) + 1) * sizeof(uint32_t) + 255) & ~size_t(255);
     const size_t need = plan_bytes + slots * (D + 2) * sizeof(float);
@@ -343,14 +345,14 @@ int launch_part(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t 
 
 bool kv_stream_supports(const KvParams& p, bool f8, int rows, uint32_t tiles_per_seq) {
     if (rows == kExPagedAny || (f8 && rows == kExContiguous)) return false;
-    const uint64_t units = uint64_t(min(p.batch, kStreamMaxBatch)) * tiles_per_seq * p.num_kv_heads * p.q_groups;
+    const uint64_t units = uint64_t(std::min(p.batch, kStreamMaxBatch)) * tiles_per_seq * p.num_kv_heads * p.q_groups;
     return units < (1ull << 31) && uint64_t(p.seq_q) * p.num_heads <= 0x7FFFFFFFu;
 }
 
 int launch_kv_stream(KvParams p, uint32_t D, bool q_f32, bool f8, int rows, uint32_t tiles_per_seq, const ScratchSource& scratch) {
     const uint32_t batch = p.batch;
     for (uint32_t b = 0; b < batch; b += kStreamMaxBatch) {  // (the parts follow each other on the stream and may share the workspace)
-        p.batch = min(batch - b, kStreamMaxBatch);
+        p.batch = std::min(batch - b, kStreamMaxBatch);
         if (int rc = launch_part(p, D, q_f32, f8, rows, tiles_per_seq, scratch)) return rc;
         if (scratch.query) break;  // the first part is the largest
         p.q = static_cast<const char*>(p.q) + size_t(p.batch) * p.q_batch * (q_f32 ? 4 : 2);

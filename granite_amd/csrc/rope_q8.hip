@@ -22,6 +22,7 @@
 // Measured (32 query heads over 8 KV heads of 128): 8187 tokens, half in and float Q out, 59.9 us a call for 256 MB, 4.3 TB/s,
 // where a large copy reaches 4.9 (66 us with one head a thread and a wave a block); 64 tokens of 64 sequences 3.2 us of
 // kernel in a call of 7.8 us: the launch; 512 tokens (64 heads) 8.4 us a call, 3.7 TB/s.
+#include <algorithm>
 #include <cmath>
 
 #include "common.h"
@@ -434,7 +435,7 @@ int launch_rope_append_q8(const granite_hip_rope_q8_args& a) {
         const uint32_t most = a.positions || a.head_dim == 64 ? kWaves : kMaxWaves;
         while (p.unit_waves < most && p.unit_waves * held < a.block_size && (p.unit_waves < kWaves || 2ull * p.unit_waves * p.kv_units <= 4096))
             p.unit_waves *= 2;
-        if (!a.positions) n_waves = max(kWaves, p.unit_waves);
+        if (!a.positions) n_waves = std::max(kWaves, p.unit_waves);
         const uint32_t per_group = a.positions ? kWaves : n_waves / p.unit_waves;
         kv_groups = (units * a.num_heads_k + per_group - 1) / per_group;
     }
