@@ -233,8 +233,8 @@ int check_form(const granite_hip_kv_form& f, const void* k, const void* v, const
     }
     p.k = static_cast<const uint8_t*>(k);
     p.v = static_cast<const uint8_t*>(v);
-    p.k_scale = f.k_scale;
-    p.v_scale = f.v_scale;
+    p.k_scale = f8 ? f.k_scale : nullptr;  // (what the pointers of a half cache hold means nothing)
+    p.v_scale = f8 ? f.v_scale : nullptr;
     p.num_blocks = f.num_blocks;
     p.block_size = table ? block_size : 1;
     p.bs_shift = (p.block_size & (p.block_size - 1)) == 0 ? __builtin_ctz(p.block_size) : -1;
