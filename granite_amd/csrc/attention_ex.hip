@@ -789,16 +789,20 @@ __global__ void __launch_bounds__(256) kv_tiles_merge_kernel(KvParams p) {
     const float inv_l = none ? 0.0f : 1.0f / l;
     const uint32_t query = row / p.group, head = kvh * p.group + row % p.group;
     const int64_t off = int64_t(query) * p.out_tok + int64_t(head) * p.out_head + 8 * dc;
+    float x[8];
+    // (a piece's infinity times a weight that has vanished is NaN here, as in the other kernels' sums)
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = settle_nan(p, o[e] * inv_l, l, 0, kvh, p.start_pos + query, p.max_tokens, 8 * dc + e);
     if constexpr (kOutF32) {
         float* op = static_cast<float*>(p.out) + off;
-        *reinterpret_cast<float4v*>(op) = float4v{o[0] * inv_l, o[1] * inv_l, o[2] * inv_l, o[3] * inv_l};
-        *reinterpret_cast<float4v*>(op + 4) = float4v{o[4] * inv_l, o[5] * inv_l, o[6] * inv_l, o[7] * inv_l};
+        *reinterpret_cast<float4v*>(op) = float4v{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<float4v*>(op + 4) = float4v{x[4], x[5], x[6], x[7]};
     } else {
         uint4v w;
-        w.x = pack_f16x2(o[0] * inv_l, o[1] * inv_l);
-        w.y = pack_f16x2(o[2] * inv_l, o[3] * inv_l);
-        w.z = pack_f16x2(o[4] * inv_l, o[5] * inv_l);
-        w.w = pack_f16x2(o[6] * inv_l, o[7] * inv_l);
+        w.x = pack_f16x2(x[0], x[1]);
+        w.y = pack_f16x2(x[2], x[3]);
+        w.z = pack_f16x2(x[4], x[5]);
+        w.w = pack_f16x2(x[6], x[7]);
         *reinterpret_cast<uint4v*>(static_cast<uint16_t*>(p.out) + off) = w;
     }
     if (p.lse && dc == 0) p.lse[int64_t(head) * p.lse_head + query] = none ? -INFINITY : (mx + __builtin_amdgcn_logf(l)) * kExLn2;

@@ -11,6 +11,39 @@ from test_gpu_kv_ex import Cache
 pytestmark = pytest.mark.gpu
 
 
+def with_infinities(rng, length, bs, hkv, d, at):
+    """A half cache with +inf in V at (token, element) of KV head 0."""
+    cache = Cache(rng, [length], bs, hkv, d, F16)
+    for token, e in at:
+        if bs:
+            cache.v[cache.table[0, token // bs] * bs + token % bs, 0, e] = np.inf
+        else:
+            cache.v[0, token, e] = np.inf
+    return cache.upload()
+
+
+def check(got, positions, window, at, group, what):
+    want = np.zeros(got.shape, bool)
+    for token, e in at:
+        sees = (token <= positions) & (token > positions - window)
+        want[sees, :group, e] = True
+    assert np.array_equal(np.isposinf(got), want), f"{what}: infinities at {np.argwhere(np.isposinf(got) != want)[0]}"
+    assert np.isfinite(got[~want]).all(), f"{what}: not finite at {np.argwhere(~np.isfinite(got) & ~want)[0]}"
+
+
+@pytest.mark.parametrize("types", [(F16, F16), (F32, F32)])
+@pytest.mark.parametrize("bs,n,hq,hkv,d", [(16, 300, 4, 1, 128), (0, 300, 4, 1, 64), (12, 300, 4, 1, 128), (16, 3, 4, 2, 64), (20, 17, 4, 1, 128)])
+def test_scores_far_apart(gpu, types, bs, n, hq, hkv, d):
+    """Scores hundreds apart: where keys are cut, the piece that holds the infinity has a weight of zero."""
+    length, window = 6000, 5000
+    at = [(1100, 3), (2900, 4), (4444, 5), (length - n, 6)]
+    cache = with_infinities(np.random.default_rng(n), length, bs, hkv, d, at)
+    q = np.random.default_rng(n + 1).standard_normal((n, hq, d)).astype(np.float16 if types[0] == F16 else np.float32)
+    got, lse = kv_ex_calls.prefill(gpu, cache, q, length - n, types[1], window, scale=100.0)
+    check(got, length - n + np.arange(n), window, at, hq // hkv, f"bs={bs} n={n}")
+    assert np.isfinite(lse).all()
+
+
 @pytest.mark.parametrize("bs,batch,hq,hkv,d", [(16, 1, 4, 2, 128), (20, 1, 4, 2, 64), (16, 24, 16, 16, 64)])
 def test_scale_pointers_of_a_half_cache_mean_nothing(gpu, bs, batch, hq, hkv, d):
     """The same form structure for both kinds of cache: k_scale and v_scale left set with kv_dtype F16."""
