@@ -136,27 +136,50 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     // ---- Q^T as B operand: lane (n, g), step s holds Q[row][16 s + 8 g .. + 7]
     half8 bq[kSteps];
     half8 bq_lo[kQF32 ? kSteps : 1];
+    float q_unit = p.scale_log2;  // kQF32: of a product with the row as loaded in the log2 domain, the K scale apart; positive
     {
         const int64_t off = int64_t(query) * p.q_tok + int64_t(head) * p.q_head + 8 * g;
+        if constexpr (kQF32) {  // as Rows16::load_q
+            const float* const qr = static_cast<const float*>(p.q) + off;
+            auto octet = [&](int s, float (&x)[8]) __attribute__((always_inline)) {
+                const float4v x0 = *reinterpret_cast<const float4v*>(qr + 16 * s), x1 = *reinterpret_cast<const float4v*>(qr + 16 * s + 4);
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) {
-            if constexpr (kQF32) {
-                const float* qp = static_cast<const float*>(p.q) + off + 16 * s;
-                const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
-                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                for (int i = 0; i < 4; i++) {
+                    x[i] = x0[i];
+                    x[4 + i] = x1[i];
+                }
+            };
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                float x[8];
+                octet(s, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+            }
+            const LanePair both = half_wave_pair(top);
+            const int shift = ex_q_shift(fmaxf(both.lo, both.hi));
+            const float power = ex_power(shift) * p.q_sign;
+            q_unit = p.scale_log2 * ex_power(-shift);
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                float x[8];
+                octet(s, x);
                 half8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xs = x[i] * p.q_sign;
+                    const float xs = x[i] * power;
                     const _Float16 h = static_cast<_Float16>(xs);
                     hi[i] = h;
                     lo[i] = static_cast<_Float16>(xs - static_cast<float>(h));
                 }
                 bq[s] = hi;
                 bq_lo[s] = lo;
-            } else {
-                bq[s] = ex_half8(*reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + off + 16 * s)) * _Float16(p.q_sign);
             }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)
+                bq[s] = ex_half8(*reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + off + 16 * s)) * _Float16(p.q_sign);
         }
     }
 
@@ -241,7 +264,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             const bool valid = r.row[f] >> 31;
             const float vs = kF8 && valid ? fminf(fmaxf(r.vs[f], 0x1p-100f), 0x1p+126f) : 1.0f;
             float4v info;
-            info.x = kF8 && valid ? fmaxf(fmaxf(r.ks[f], 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
+            // (float queries: the K scale alone, each row has a factor of its own)
+            if constexpr (kQF32) info.x = kF8 && valid ? fmaxf(r.ks[f], 0x1p-126f) : 1.0f;
+            else info.x = kF8 && valid ? fmaxf(fmaxf(r.ks[f], 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
             info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
             info.z = 1.0f / vs;
             info.w = valid ? 1.0f : 0.0f;
@@ -344,11 +369,15 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         uint32_t bits;  // of those whose page is one of the pool's
     };
     constexpr uint32_t kAllRuns = (1u << kLaneRuns) - 1;
+    // positive and finite, so that a masked score stays minus infinity and a product of zero stays zero
+    auto factor_of = [&](float ks) __attribute__((always_inline)) {
+        return kQF32 ? __builtin_amdgcn_fmed3f(ks * q_unit, 0x1p-126f, FLT_MAX) : q_unit;
+    };
     auto runs_of = [&](uint32_t it, int sub) __attribute__((always_inline)) -> Runs {
         Runs x;
         x.bits = kAllRuns;
         if constexpr (kRows == kExContiguous) {
-            x.r[0] = x.r[1] = Run{p.scale_log2, 0.0f, 1.0f};
+            x.r[0] = x.r[1] = Run{factor_of(1.0f), 0.0f, 1.0f};
         } else {
             const uint32_t at = (it - t_begin) % (2 * kPlan) * kTileRuns + (kTileRuns / 2) * sub + (kFine ? g : 0);
             x.bits = 0;
@@ -356,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             for (int a = 0; a < kLaneRuns; a++) {
                 const float4v r = s_run[at + (kFine ? 2 * a : a)];
                 x.bits |= r.w != 0.0f ? 1u << a : 0u;
-                x.r[a] = kF8 ? Run{r.x, r.y, r.z} : Run{p.scale_log2, 0.0f, 1.0f};
+                x.r[a] = kF8 ? Run{kQF32 ? factor_of(r.x) : r.x, r.y, r.z} : Run{factor_of(1.0f), 0.0f, 1.0f};
             }
             if constexpr (!kFine) x.bits = ex_uniform(x.bits);
         }

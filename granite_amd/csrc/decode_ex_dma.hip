@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
 
     // ---- query rows and running state, as Rows16
     half8 bq[kSteps], bq_lo[kQF32 ? kSteps : 1];
+    float q_unit = p.scale_log2;  // of a product with the row as loaded in the log2 domain, the K scale apart
     float m_run = kExNegBig, l_run = 0.0f, vref = 0x1p-100f, inv_vref = 0x1p+100f;
     float4v acc[kBlocks];
     auto clear = [&]() __attribute__((always_inline)) {
@@ -284,25 +285,47 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
             row_hi = all_hi = u.len;
             row_lo = all_lo = window_begin(u.len - 1, p.window);
         }
+        auto d_of = [&](int s) __attribute__((always_inline)) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); };
+        if constexpr (kQF32) {  // as Rows16::load_q
+            const float* const qr = static_cast<const float*>(p.q) + at;
+            auto octet = [&](int s, float (&x)[8]) __attribute__((always_inline)) {
+                const float4v x0 = *reinterpret_cast<const float4v*>(qr + d_of(s)), x1 = *reinterpret_cast<const float4v*>(qr + d_of(s) + 4);
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) {
-            const int64_t off = at + 64 * (s / 2) + 16 * g + 8 * (s % 2);
-            if constexpr (kQF32) {
-                const float* qp = static_cast<const float*>(p.q) + off;
-                const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
-                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                for (int i = 0; i < 4; i++) {
+                    x[i] = x0[i];
+                    x[4 + i] = x1[i];
+                }
+            };
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                float x[8];
+                octet(s, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+            }
+            const int shift = ex_q_shift(max_over_groups(top));
+            const float power = ex_power(shift);
+            q_unit = p.scale_log2 * ex_power(-shift);
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                float x[8];
+                octet(s, x);
                 half8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xv = live ? x[i] : 0.0f;
+                    const float xv = live ? x[i] * power : 0.0f;
                     const _Float16 h = static_cast<_Float16>(xv);
                     hi[i] = h;
                     lo[i] = static_cast<_Float16>(xv - static_cast<float>(h));
                 }
                 bq[s] = hi;
                 bq_lo[s] = lo;
-            } else {
-                uint4v w = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + off);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                uint4v w = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + at + d_of(s));
                 if (!live) w = uint4v{0, 0, 0, 0};
                 bq[s] = ex_half8(w);
             }
@@ -370,7 +393,7 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
 #pragma unroll
         for (int sub = 0; sub < 2; sub++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[sub][i] = c[sub][i] * (u.ks[sub] * p.scale_log2);
+            for (int i = 0; i < 4; i++) s[sub][i] = c[sub][i] * ex_finite(u.ks[sub] * q_unit);
         uint32_t sees = 0xFFu;  // kMulti: bit 4 sub + i, the lane's row sees token 16 sub + 4 g + i
         const bool masked = u.tok + kTokens > all_hi || (u.tok < all_lo && u.tok + kTokens > p.sinks) || u.valid != 3;
         if (masked) {

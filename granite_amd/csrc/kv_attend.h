@@ -2,6 +2,8 @@
 // attention_ex.hip): the launch parameters and the work of one wave on one key tile.
 #pragma once
 
+#include <cfloat>
+
 #include "common.h"
 #include "kv_choice.h"
 #include "kv_visible.h"
@@ -300,13 +302,30 @@ struct Tile {
     }
 };
 
-// Query rows of a wave as B operands, and the running softmax state of those rows.  Float queries
-// are a half and a half remainder: nothing of them is lost.
+// The maximum over the four lanes n, n + 16, n + 32, n + 48, in all of them: two register swaps, no LDS round trip
+// (v_permlane16_swap exchanges the odd rows of 16 lanes of one register with the even rows of the other).
+__device__ __forceinline__ float max_over_groups(float v) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    const LanePair both = half_wave_pair(fmaxf(a, b));
+    return fmaxf(both.lo, both.hi);
+}
+
+// Float queries are taken times a power of two, the same for a whole row, that brings the row's largest element, `top`, to
+// 2^14 .. 2^15, and then as a half and a half remainder: an element is off by at most 2^-23 of itself or 2^-40 of the largest,
+// whatever the row's magnitude (2^-97 and more).  The scores' factor takes the power back.  Infinities and NaN stay what they are.
+__device__ __forceinline__ int ex_q_shift(float top) { return max(-113, min(112, 15 - __builtin_amdgcn_frexp_expf(top))); }
+__device__ __forceinline__ float ex_power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
+// A factor of scores as a finite number: a code of zero times it is zero.
+__device__ __forceinline__ float ex_finite(float x) { return fminf(fmaxf(x, -FLT_MAX), FLT_MAX); }
+
+// Query rows of a wave as B operands, and the running softmax state of those rows.
 template <bool kQF32, bool kF8, int kD>
 struct Rows16 {
     static constexpr int kSteps = kD / 32;
     half8 bq[kSteps];
     half8 bq_lo[kQF32 ? kSteps : 1];
+    float unit;   // of a product with the row as loaded in the log2 domain, the K scale apart
     float m, l;   // running maximum (log2 domain) and this lane's part of the sum
     float vref, inv_vref;  // V scale the accumulators are relative to (from the start one whose inverse leaves room
                            // for kExBoost: a tile of nothing but masked runs multiplies it by zero)
@@ -322,26 +341,48 @@ struct Rows16 {
     }
     // src: element offset of the lane's row; dead rows are zeros
     __device__ __forceinline__ void load_q(const KvParams& p, int64_t at, bool live, uint32_t g) {
+        if constexpr (kQF32) {
+            const float* const row = static_cast<const float*>(p.q) + at;
+            auto octet = [&](int s, float (&x)[8]) __attribute__((always_inline)) {
+                const float* qp = row + Tile<kF8, kExContiguous, kD>::d_of(s, g);
+                const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
 #pragma unroll
-        for (int s = 0; s < kSteps; s++) {
-            const int64_t off = at + Tile<kF8, kExContiguous, kD>::d_of(s, g);
-            if constexpr (kQF32) {
-                const float* qp = static_cast<const float*>(p.q) + off;
-                const float4v x0 = *reinterpret_cast<const float4v*>(qp);
-                const float4v x1 = *reinterpret_cast<const float4v*>(qp + 4);
-                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                for (int i = 0; i < 4; i++) {
+                    x[i] = x0[i];
+                    x[4 + i] = x1[i];
+                }
+            };
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                float x[8];
+                octet(s, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+            }
+            const int shift = ex_q_shift(max_over_groups(top));
+            const float power = ex_power(shift);
+            unit = p.scale_log2 * ex_power(-shift);
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                float x[8];
+                octet(s, x);
                 half8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xv = live ? x[i] : 0.0f;
+                    const float xv = live ? x[i] * power : 0.0f;
                     const _Float16 h = static_cast<_Float16>(xv);
                     hi[i] = h;
                     lo[i] = static_cast<_Float16>(xv - static_cast<float>(h));
                 }
                 bq[s] = hi;
                 bq_lo[s] = lo;
-            } else {
-                uint4v w = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + off);
+            }
+        } else {
+            unit = p.scale_log2;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                uint4v w = *reinterpret_cast<const uint4v*>(static_cast<const uint16_t*>(p.q) + at + Tile<kF8, kExContiguous, kD>::d_of(s, g));
                 if (!live) w = uint4v{0, 0, 0, 0};
                 bq[s] = ex_half8(w);
             }
@@ -370,15 +411,6 @@ __device__ __forceinline__ float settle_nan(const KvParams& p, float result, flo
         if (!(fabsf(x) < INFINITY)) sum += x;
     }
     return sum != 0.0f ? sum : result;
-}
-
-// The maximum over the four lanes n, n + 16, n + 32, n + 48, in all of them: two register swaps, no LDS round trip
-// (v_permlane16_swap exchanges the odd rows of 16 lanes of one register with the even rows of the other).
-__device__ __forceinline__ float max_over_groups(float v) {
-    float a = v, b = v;
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    const LanePair both = half_wave_pair(fmaxf(a, b));
-    return fmaxf(both.lo, both.hi);
 }
 
 // One tile's contribution to the rows of `st`.  `seen` is what all rows see between them, [lo, hi) and
@@ -413,7 +445,7 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
             if constexpr (kQF32) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, st.bq_lo[step], c, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[sub][i] = c[i] * (kF8 ? of_token(rows.ks, sub, i) * p.scale_log2 : p.scale_log2);
+        for (int i = 0; i < 4; i++) s[sub][i] = c[i] * ex_finite(kF8 ? of_token(rows.ks, sub, i) * st.unit : st.unit);
     }
     bool special = false;  // kPerRow, masked: some V of the tile is infinite or NaN
     uint32_t visible = 0xFFFFu;  // bit 4 sub + i: the lane's row sees token 16 sub + 4 g + i

@@ -481,9 +481,10 @@ int granite_hip_matvec_q4k_batched(const void *x, int64_t x_stride, const void *
  *     a log-sum-exp of minus infinity;
  *   - K or V values of tokens that a query does not see never reach its result, also where they are
  *     NaN or infinite.
- * Probabilities, sums and accumulators are float; decode and float outputs carry float precision
- * (probabilities enter the second product as a half and a half remainder), half outputs take
- * probabilities rounded to half. */
+ * Sums and accumulators are float.  Probabilities enter the second product as a half and a half remainder,
+ * 22 bits; with half outputs and many rows as one half.  A row (token and head) of float queries is scaled by
+ * a power of two and split into a half and a half remainder: an element of a row of any magnitude counts to
+ * within 2^-23 of itself or 2^-40 of the row's largest, whichever is more. */
 typedef struct granite_hip_kv_form {
     int kv_dtype;         /* GRANITE_HIP_F16 or GRANITE_HIP_F8E4M3 (paged pools only) */
     const float *k_scale; /* F8E4M3: float[num_blocks, num_kv_heads] */

@@ -97,3 +97,60 @@ def compare(got, got_lse, want, what):
     assert len(bad) == 0, f"{what}: {len(bad)} of {out.size} off, first {bad[0]}: {got[tuple(bad[0])]} for {out[tuple(bad[0])]}, allowed {tol[tuple(bad[0])]}"
     bad = np.argwhere(off_lse > tol_lse)
     assert len(bad) == 0, f"{what}: lse {bad[0]}: {got_lse[tuple(bad[0])]} for {lse[tuple(bad[0])]}"
+
+
+# (kv, block size, heads, KV heads, head size, lengths, window and sinks, sequences that are looked at): decode steps of the row
+# kernel (with and without runs of 16 tokens), of the persistent one over 8-bit pools, and of the one over half pools
+STEPS = {
+    "rows": (F8E4M3, 16, 8, 2, 128, [700, 33, 600], (0, 0), (0, 1, 2)),
+    "rows any block": (F8E4M3, 20, 8, 2, 64, [700, 33, 600], (0, 0), (0, 1, 2)),
+    "rows half": (F16, 16, 8, 2, 128, [700, 33, 600], (500, 4), (0, 1, 2)),
+    "rows half any block": (F16, 12, 8, 2, 64, [700, 33, 600], (500, 4), (0, 2)),
+    "persistent 8-bit": (F8E4M3, 16, 16, 16, 64, [2500, 31, 32, 33] + [600] * 20, (0, 0), (0, 1, 2, 3, 23)),
+    "persistent 8-bit 128": (F8E4M3, 64, 32, 8, 128, [2900, 31, 2899, 33] + [300] * 20, (0, 0), (0, 1, 2, 3, 23)),
+    "persistent half": (F16, 16, 16, 8, 128, [4000, 31, 3999, 33] + [300] * 12, (3900, 4), (0, 1, 2, 3)),
+}
+# (kv, block size, heads, KV heads, head size, queries, first position, window and sinks, queries that are looked at, tiles kernel)
+RUNS = {
+    "rows": (F8E4M3, 16, 8, 2, 128, 5, 595, (0, 0), (0, 1, 4), False),
+    "rows any block": (F8E4M3, 5, 8, 2, 64, 5, 595, (0, 0), (0, 1, 4), False),
+    "rows half": (F16, 0, 8, 2, 128, 5, 595, (400, 4), (0, 1, 4), False),
+    "persistent": (F8E4M3, 48, 16, 2, 128, 3, 8100, (0, 0), (0, 1, 2), False),
+    "tiles": (F8E4M3, 16, 96, 1, 64, 420, 480, (0, 0), (0, 33, 34, 419), True),
+    "tiles 128": (F8E4M3, 16, 96, 1, 128, 420, 480, (0, 0), (0, 419), True),
+    "tiles any block": (F8E4M3, 20, 96, 1, 64, 420, 480, (300, 4), (0, 33, 419), True),
+    "tiles half": (F16, 16, 96, 1, 128, 420, 480, (300, 4), (0, 33, 419), True),
+    "tiles contiguous": (F16, 0, 96, 1, 64, 420, 480, (300, 4), (0, 419), True),
+    "tiles cut": (F8E4M3, 16, 8, 1, 64, 400, 5000, (0, 0), (0, 399), True),
+}
+
+
+@functools.lru_cache(maxsize=20)
+def made(kv, bs, hkv, d, lens):
+    return Cache(np.random.default_rng(1), lens, bs, hkv, d, kv)
+
+
+def step_cache(name):
+    kv, bs, hq, hkv, d, lens, window, some = STEPS[name]
+    return copy.deepcopy(made(kv, bs, hkv, d, tuple(lens))), (len(lens), hq, d), window, some
+
+
+def run_cache(name):
+    kv, bs, hq, hkv, d, n, start, window, some, tiles = RUNS[name]
+    return copy.deepcopy(made(kv, bs, hkv, d, (start + n,))), (n, hq, d), start, window, some, tiles
+
+
+def check_step(gpu, cache, q, window, some, scale=None, what=""):
+    got, lse = decode(gpu, cache, q, *window, scale=scale)
+    for i in some:
+        want = reference(cache, i, q[i:i + 1], [cache.lens[i] - 1], *window, scale)
+        compare(got[i:i + 1], lse[i:i + 1], want, f"{what} sequence {i}")
+    return got, lse
+
+
+def check_run(gpu, cache, q, start, window, some, tiles, out_dtype, scale=None, what=""):
+    some = np.asarray(some)
+    got, lse = prefill(gpu, cache, q, start, out_dtype, *window, scale=scale)
+    want = reference(cache, 0, q[some], start + some, *window, scale, tiles=tiles, half=out_dtype == F16)
+    compare(got[some], lse[some], want, what)
+    return got, lse
