@@ -141,34 +141,32 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         const int64_t off = int64_t(query) * p.q_tok + int64_t(head) * p.q_head + 8 * g;
         if constexpr (kQF32) {  // as Rows16::load_q
             const float* const qr = static_cast<const float*>(p.q) + off;
-            auto octet = [&](int s, float (&x)[8]) __attribute__((always_inline)) {
-                const float4v x0 = *reinterpret_cast<const float4v*>(qr + 16 * s), x1 = *reinterpret_cast<const float4v*>(qr + 16 * s + 4);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[i] = x0[i];
-                    x[4 + i] = x1[i];
-                }
-            };
-            float top = 0.0f;
+            float x[kSteps][8];
 #pragma unroll
             for (int s = 0; s < kSteps; s++) {
-                float x[8];
-                octet(s, x);
+                const float* qp = qr + 16 * s;
+                const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
 #pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+                for (int i = 0; i < 4; i++) {
+                    x[s][i] = x0[i];
+                    x[s][4 + i] = x1[i];
+                }
             }
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[s][i]));
             const LanePair both = half_wave_pair(top);
             const int shift = ex_q_shift(fmaxf(both.lo, both.hi));
             const float power = ex_power(shift) * p.q_sign;
             q_unit = p.scale_log2 * ex_power(-shift);
 #pragma unroll
             for (int s = 0; s < kSteps; s++) {
-                float x[8];
-                octet(s, x);
                 half8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xs = x[i] * power;
+                    const float xs = x[s][i] * power;
                     const _Float16 h = static_cast<_Float16>(xs);
                     hi[i] = h;
                     lo[i] = static_cast<_Float16>(xs - static_cast<float>(h));

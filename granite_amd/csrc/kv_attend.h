@@ -343,34 +343,31 @@ struct Rows16 {
     __device__ __forceinline__ void load_q(const KvParams& p, int64_t at, bool live, uint32_t g) {
         if constexpr (kQF32) {
             const float* const row = static_cast<const float*>(p.q) + at;
-            auto octet = [&](int s, float (&x)[8]) __attribute__((always_inline)) {
+            float x[kSteps][8];
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
                 const float* qp = row + Tile<kF8, kExContiguous, kD>::d_of(s, g);
                 const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    x[i] = x0[i];
-                    x[4 + i] = x1[i];
+                    x[s][i] = x0[i];
+                    x[s][4 + i] = x1[i];
                 }
-            };
+            }
             float top = 0.0f;
 #pragma unroll
-            for (int s = 0; s < kSteps; s++) {
-                float x[8];
-                octet(s, x);
+            for (int s = 0; s < kSteps; s++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
-            }
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[s][i]));
             const int shift = ex_q_shift(max_over_groups(top));
             const float power = ex_power(shift);
             unit = p.scale_log2 * ex_power(-shift);
 #pragma unroll
             for (int s = 0; s < kSteps; s++) {
-                float x[8];
-                octet(s, x);
                 half8 hi, lo;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float xv = live ? x[i] * power : 0.0f;
+                    const float xv = live ? x[s][i] * power : 0.0f;
                     const _Float16 h = static_cast<_Float16>(xv);
                     hi[i] = h;
                     lo[i] = static_cast<_Float16>(xv - static_cast<float>(h));
