@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kRowWaves* kWave, 2) kv_rows_kernel(KvParams p
             s_ml[wave][n][0] = st.m;
             s_ml[wave][n][1] = l;
         }
-        const float unit = st.vref * (1.0f / kExBoost);
+        const float unit = ex_unit(st.bound);
         if (32 * g < uint32_t(kD)) {
 #pragma unroll
             for (int e = 0; e < 32; e++) s_o(wave, n, 32 * g + e) = st.acc[e & 7][e >> 3] * unit;

@@ -254,13 +254,12 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
     // ---- query rows and running state, as Rows16
     half8 bq[kSteps], bq_lo[kQF32 ? kSteps : 1];
     float q_unit = p.scale_log2;  // of a product with the row as loaded in the log2 domain, the K scale apart
-    float m_run = kExNegBig, l_run = 0.0f, vref = 0x1p-100f, inv_vref = 0x1p+100f;
+    float m_run = kExNegBig, l_run = 0.0f, bound = kExNegBig;
     float4v acc[kBlocks];
     auto clear = [&]() __attribute__((always_inline)) {
         m_run = kExNegBig;
         l_run = 0.0f;
-        vref = 0x1p-100f;
-        inv_vref = 0x1p+100f;
+        bound = kExNegBig;
 #pragma unroll
         for (int t = 0; t < kBlocks; t++) acc[t] = float4v{0, 0, 0, 0};
     };
@@ -337,7 +336,7 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
         if (row0 + n < n_rows) {
             const uint32_t piece = worker + u.b * lists + lh;
             const size_t at = size_t(piece) * p.part_cap + (wave % kPer) * (p.part_cap / kPer) + n;
-            const float unit = vref * (1.0f / kExBoost);
+            const float unit = ex_unit(bound);
 #pragma unroll
             for (int t = 0; t < kBlocks; t++) *reinterpret_cast<float4v*>(p.part_o + at * kD + 16 * t + 4 * g) = acc[t] * unit;
             if (g == 0) {
@@ -419,33 +418,31 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
                 asm volatile("" : "+v"(vw[t]));
             }
         }
-        float top = s[0][0];
+        float tops[2];
 #pragma unroll
-        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i / 4][i % 4]);
-        top = max_over_groups(top);
-        const float m_new = fmaxf(m_run, top);
-        float rescale = fast_exp2(m_run - m_new);
-        l_run *= rescale;
-        const float vmax = fmaxf(u.vs[0], u.vs[1]);
-        if (__any(vmax > vref)) {  // the same in every lane
-            rescale *= vref / vmax;
-            vref = vmax;
-            inv_vref = 1.0f / vmax;
-        }
+        for (int sub = 0; sub < 2; sub++) tops[sub] = fmaxf(fmaxf(s[sub][0], s[sub][1]), fmaxf(s[sub][2], s[sub][3]));
+        const float top = max_over_groups(fmaxf(tops[0], tops[1])), m_new = fmaxf(m_run, top), moved = m_run - m_new;
+        m_run = m_new;
+        l_run *= fast_exp2(moved);
+        // V scales relative to the row's largest p * (V scale), as attend_tile
+        const float e0 = ex_exponent(u.vs[0]), e1 = ex_exponent(u.vs[1]);
+        const float z = max_over_groups(fmaxf((tops[0] - m_new) + e0, (tops[1] - m_new) + e1));
+        const float bound_new = fmaxf(bound + moved, z), whole = ceilf(bound_new);
+        const float rescale = fast_exp2(moved + (ceilf(bound) - whole));
+        bound = bound_new;
         if (__any(rescale != 1.0f)) {
 #pragma unroll
             for (int t = 0; t < kBlocks; t++) acc[t] *= rescale;
         }
-        m_run = m_new;
         half8 hi, rem;
 #pragma unroll
         for (int sub = 0; sub < 2; sub++) {
-            const float f = u.vs[sub] * (inv_vref * kExBoost);
+            const float shift = (sub ? e1 : e0) - whole, f = ex_mantissa(u.vs[sub]) * kExBoost;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float e = fast_exp2(s[sub][i] - m_new);
-                l_run += e;
-                const float scaled = e * f;
+                const float d = s[sub][i] - m_new;
+                l_run += fast_exp2(d);
+                const float scaled = fast_exp2(d + shift) * f;
                 const _Float16 h = static_cast<_Float16>(scaled);
                 hi[4 * sub + i] = h;
                 rem[4 * sub + i] = static_cast<_Float16>(scaled - static_cast<float>(h));

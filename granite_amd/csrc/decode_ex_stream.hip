@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_stream_kernel(KvParams p)
             const uint32_t piece = worker + of_unit(d_b, i) * lists + lh;
             const size_t at = size_t(piece) * p.part_cap + (wave % kPer) * (p.part_cap / kPer) + n;
             float* po = p.part_o + at * kD + 32 * g;
-            const float unit = st.vref * (1.0f / kExBoost);
+            const float unit = ex_unit(st.bound);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 float4v w;

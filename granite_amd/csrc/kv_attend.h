@@ -83,10 +83,20 @@ __device__ __forceinline__ half8 f8x8_to_half8(uint32_t a, uint32_t b) {
     return ex_half8(uint4v{f8x2_to_f16x2<false>(a), f8x2_to_f16x2<true>(a), f8x2_to_f16x2<false>(b), f8x2_to_f16x2<true>(b)});
 }
 
-// Probabilities enter the second product times this: with V scales taken relative to the largest one
-// seen (ratios <= 1) a factor of 2^14 keeps the products of small ratios and probabilities in the normal range of
-// a half, 65504 being out of reach.
+// Probabilities enter the second product times this, and over 8-bit pools times the V scale over 2^bound, where 2^bound is the
+// largest p * (V scale) among the keys that the row itself has seen: it is then near 2^14, 65504 being out of reach, and what is
+// up to 2^28 times smaller keeps 22 bits in a half and its remainder.  The scale goes into the exponent of the
+// probability, which by itself might vanish.  (The bound has to follow the probabilities: taken from the scales alone, a
+// block of next to no probability whose scale is 2^40 times the others' left nothing of these.  One for the wave with a
+// change to one for every row where scales lie 2^7 apart is as quick.)
 constexpr float kExBoost = 16384.0f;
+
+__device__ __forceinline__ float ex_power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
+// A V scale as mantissa (0.5 <= . < 1) and exponent.
+__device__ __forceinline__ float ex_exponent(float vs) { return float(__builtin_amdgcn_frexp_expf(vs)); }
+__device__ __forceinline__ float ex_mantissa(float vs) { return __builtin_amdgcn_frexp_mantf(vs); }
+// What an accumulator relative to `bound` (log2, see Rows16) counts.
+__device__ __forceinline__ float ex_unit(float bound) { return __builtin_ldexpf(1.0f / kExBoost, int(fmaxf(ceilf(bound), -200.0f))); }
 
 __device__ __forceinline__ uint32_t ex_seq_len(const KvParams& p, uint32_t b) {
     const uint32_t len = p.seq_lens ? uint32_t(max(p.seq_lens[b], 0)) : p.max_tokens;
@@ -315,7 +325,6 @@ __device__ __forceinline__ float max_over_groups(float v) {
 // 2^14 .. 2^15, and then as a half and a half remainder: an element is off by at most 2^-23 of itself or 2^-40 of the largest,
 // whatever the row's magnitude (2^-97 and more).  The scores' factor takes the power back.  Infinities and NaN stay what they are.
 __device__ __forceinline__ int ex_q_shift(float top) { return max(-113, min(112, 15 - __builtin_amdgcn_frexp_expf(top))); }
-__device__ __forceinline__ float ex_power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 // A factor of scores as a finite number: a code of zero times it is zero.
 __device__ __forceinline__ float ex_finite(float x) { return fminf(fmaxf(x, -FLT_MAX), FLT_MAX); }
 
@@ -327,15 +336,14 @@ struct Rows16 {
     half8 bq_lo[kQF32 ? kSteps : 1];
     float unit;   // of a product with the row as loaded in the log2 domain, the K scale apart
     float m, l;   // running maximum (log2 domain) and this lane's part of the sum
-    float vref, inv_vref;  // V scale the accumulators are relative to (from the start one whose inverse leaves room
-                           // for kExBoost: a tile of nothing but masked runs multiplies it by zero)
+    float bound;  // 8 bits: log2 of the largest p * 2^(exponent of the V scale), p relative to m; acc counts in units of
+                  // 2^ceil(bound) / kExBoost: whole powers of two, which are taken off an exponent without a rounding
     float4v acc[8];
 
     __device__ __forceinline__ void clear() {
         m = kExNegBig;
         l = 0.0f;
-        vref = kF8 ? 0x1p-100f : 1.0f;
-        inv_vref = kF8 ? 0x1p+100f : 1.0f;
+        bound = kF8 ? kExNegBig : 0.0f;
 #pragma unroll
         for (int t = 0; t < 8; t++) acc[t] = float4v{0, 0, 0, 0};
     }
@@ -487,25 +495,27 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
 #pragma unroll
     for (int i = 1; i < 4 * kSubs; i++) top = fmaxf(top, s[i / 4][i % 4]);
     top = max_over_groups(top);
-    const float m_new = fmaxf(st.m, top);
-    float rescale = fast_exp2(st.m - m_new);  // of O; of l without the change of the V scale
+    const float m_new = fmaxf(st.m, top), moved = st.m - m_new;
+    float rescale = fast_exp2(moved), whole = 0.0f;  // of O, of l; ceil(bound)
     st.l *= rescale;
     if constexpr (kF8) {
-        float vmax = rows.vs;
-        if constexpr (kRows == kExPaged16) {
+        float z = -INFINITY;
 #pragma unroll
-            for (int sub = 0; sub < kSubs; sub++) vmax = fmaxf(vmax, of_token(rows.vs, sub, 0));
-        } else {
+        for (int sub = 0; sub < kSubs; sub++) {
+            if constexpr (kRows == kExPaged16) {
+                const float t = fmaxf(fmaxf(s[sub][0], s[sub][1]), fmaxf(s[sub][2], s[sub][3]));
+                z = fmaxf(z, (t - m_new) + ex_exponent(of_token(rows.vs, sub, 0)));
+            } else {
 #pragma unroll
-            for (int off = 1; off < 64; off <<= 1) vmax = fmaxf(vmax, wave_shfl_xor(vmax, off));
+                for (int i = 0; i < 4; i++) z = fmaxf(z, (s[sub][i] - m_new) + ex_exponent(of_token(rows.vs, sub, i)));
+            }
         }
-        if (__any(vmax > st.vref)) {  // the same in every lane
-            rescale *= st.vref / vmax;
-            st.vref = vmax;
-            st.inv_vref = 1.0f / vmax;
-        }
+        const float bound = fmaxf(st.bound + moved, max_over_groups(z));
+        whole = ceilf(bound);
+        rescale = fast_exp2(moved + (ceilf(st.bound) - whole));
+        st.bound = bound;
     }
-    if (__any(m_new > st.m || rescale != 1.0f)) {
+    if (__any(rescale != 1.0f)) {
 #pragma unroll
         for (int t = 0; t < 8; t++) st.acc[t] *= rescale;
     }
@@ -515,9 +525,13 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
     for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float e = fast_exp2(s[sub][i] - m_new);
+            const float d = s[sub][i] - m_new, e = fast_exp2(d);
             st.l += e;
-            const float scaled = e * (kF8 ? of_token(rows.vs, sub, i) * (st.inv_vref * kExBoost) : kExBoost);
+            float scaled = e * kExBoost;
+            if constexpr (kF8) {
+                const float vs = of_token(rows.vs, sub, i);
+                scaled = fast_exp2(d + (ex_exponent(vs) - whole)) * (ex_mantissa(vs) * kExBoost);
+            }
             const _Float16 h = static_cast<_Float16>(scaled);
             hi8[sub / 2][4 * (sub % 2) + i] = h;
             lo8[sub / 2][4 * (sub % 2) + i] = static_cast<_Float16>(scaled - static_cast<float>(h));
