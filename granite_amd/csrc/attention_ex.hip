@@ -46,6 +46,7 @@ constexpr int kThreads = 512;
 constexpr int kKBuffers = 3, kVBuffers = 3;
 constexpr uint32_t kPlan = 64;  // tiles whose rows and scales are worked out at a time
 constexpr float kProbLimit = 16384.0f;  // a row's probabilities of a sub-tile may sum to this much
+constexpr float kFusedScores = 0x1p20f;  // references below this leave scores to a fused multiply-add
 
 template <int kD, int kRows>
 struct Shape {
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         }
     }
 
-    float m_ref = kExNegBig, l_run = 0.0f;
+    float m_ref = kExNegBig, l_run = 0.0f, limit = kProbLimit;
     float16v oacc[kBlocks];
 #pragma unroll
     for (int t = 0; t < kBlocks; t++)
@@ -421,15 +422,23 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         half8 lo[kPrecise ? 2 : 1];
     };
     // Probabilities are relative to a reference that moves only when those of a sub-tile sum to kProbLimit or more
-    // (or to infinity, as in the first), see prefill.hip.
+    // (or to infinity, as in the first), see prefill.hip.  In front of the exponential a score is fused with its
+    // factor and the reference.  What the reference's own rounding leaves there, up to half its last place, is nothing while
+    // it is below 2^20 but beyond a float's exponents from 2^30 on: a row whose reference is that large has every sub-tile done
+    // again with rounded scores (limit 0), whose difference to the reference is exact.
+    auto rounded_score = [&](float s, float scale) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
+        return s * scale;
+    };
     auto rebase = [&](const float16v& s, const Runs& runs) __attribute__((always_inline)) {
         float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 16; r++) top = fmaxf(top, __builtin_fmaf(s[r], runs.r[r >> kRunShift].scale, runs.r[r >> kRunShift].lvs));
+        for (int r = 0; r < 16; r++) top = fmaxf(top, rounded_score(s[r], runs.r[r >> kRunShift].scale) + runs.r[r >> kRunShift].lvs);
         const LanePair both = half_wave_pair(top);
         const float m_new = fmaxf(m_ref, fmaxf(both.lo, both.hi));
         const float alpha = fast_exp2(m_ref - m_new);
         m_ref = m_new;
+        limit = fabsf(m_ref) < kFusedScores || m_ref == kExNegBig ? kProbLimit : 0.0f;
         l_run *= alpha;
 #pragma unroll
         for (int t = 0; t < kBlocks; t++)
@@ -454,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int a = (8 * u + j) >> kRunShift;
-                pe[j] = fast_exp2(__builtin_fmaf(s[8 * u + j], runs.r[a].scale, runs.r[a].lvs - m_ref));
+                pe[j] = fast_exp2((rounded_score(s[8 * u + j], runs.r[a].scale) - m_ref) + runs.r[a].lvs);
                 sum[a] += pe[j];
             }
             pack(pe, out.hi[u], &out.lo[kPrecise ? u : 0]);
@@ -549,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             p_out.lo[0] = ex_half8(uint4v{pl[0], pl[1], pl[2], pl[3]});
             p_out.lo[1] = ex_half8(uint4v{pl[4], pl[5], pl[6], pl[7]});
         }
-        if (__any(!(total_of(psum) < kProbLimit))) {  // rare: the reference has to move, redo the sub-tile
+        if (__any(!(total_of(psum) < limit))) {  // rare: the reference has to move, redo the sub-tile
             rebase(s_in, runs_in);
             probabilities_once(s_in, runs_in, p_out, psum);
         }

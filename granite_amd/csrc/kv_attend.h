@@ -12,7 +12,7 @@ namespace ghip {
 
 constexpr float kExLog2e = 1.4426950408889634f;
 constexpr float kExLn2 = 0.6931471805599453f;
-constexpr float kExNegBig = -1.0e30f;
+constexpr float kExNegBig = -FLT_MAX;  // what a running maximum starts from: at or below any finite score
 
 // How token positions map to rows.  Runs of 16 consecutive tokens that start at a multiple of 16 lie in
 // one block when the block size is a multiple of 16: one table entry, one scale and one base address

@@ -478,7 +478,7 @@ int granite_hip_matvec_q4k_batched(const void *x, int64_t x_stride, const void *
  *     Under a window, entries of blocks that hold neither a token of the window nor a sink are not
  *     used at all, so a caller can release those blocks and leave the entries stale;
  *   - a query that sees no key (its window lies behind the cache, every page invalid) gets zeros and
- *     a log-sum-exp of minus infinity;
+ *     a log-sum-exp of minus infinity, as does one all of whose scores are minus infinity;
  *   - K or V values of tokens that a query does not see never reach its result, also where they are
  *     NaN or infinite.
  * Sums and accumulators are float.  Probabilities enter the second product as a half and a half remainder,
