@@ -46,6 +46,7 @@ constexpr int kThreads = 512;
 constexpr int kKBuffers = 3, kVBuffers = 3;
 constexpr uint32_t kPlan = 64;  // tiles whose rows and scales are worked out at a time
 constexpr float kProbLimit = 16384.0f;  // a row's probabilities of a sub-tile may sum to this much
+constexpr float kPlainScales = 48.0f;   // V scales within 2^-48 .. 2^48 take the sum's weights from the probabilities
 constexpr float kFusedScores = 0x1p20f;  // references below this leave scores to a fused multiply-add
 
 template <int kD, int kRows>
@@ -86,7 +87,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     extern __shared__ __attribute__((aligned(16))) uint16_t s_mem[];
     uint16_t* const s_k0 = s_mem;
     uint16_t* const s_v0 = s_mem + kKBuffers * kKTile;
-    // of run i of the workgroup's j-th tile, at (j mod 128) * kTileRuns + i: scale of the scores, log2 of the V scale, its inverse, valid
+    // of run i of the workgroup's j-th tile, at (j mod 128) * kTileRuns + i: scale of the scores, log2 of the V scale, its inverse,
+    // 0 (no page of the pool's), 1 or 2 (a V scale beyond 2^+-kPlainScales)
     float4v* const s_run = reinterpret_cast<float4v*>(reinterpret_cast<unsigned char*>(s_mem) + S::kTileBytes);
     uint32_t* const s_special = reinterpret_cast<uint32_t*>(s_run + 2 * kPlan * kTileRuns);
 
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             else info.x = kF8 && valid ? fmaxf(fmaxf(r.ks[f], 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
             info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
             info.z = 1.0f / vs;
-            info.w = valid ? 1.0f : 0.0f;
+            info.w = !valid ? 0.0f : fabsf(info.y) > kPlainScales ? 2.0f : 1.0f;
             s_run[(half * kPlan + lane) * kTileRuns + (kFine ? 2 * wave + f : wave >> 1)] = info;
         }
     };
@@ -366,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     struct Runs {
         Run r[kLaneRuns];
         uint32_t bits;  // of those whose page is one of the pool's
+        bool far;       // one has a V scale beyond 2^+-kPlainScales
     };
     constexpr uint32_t kAllRuns = (1u << kLaneRuns) - 1;
     // positive and finite, so that a masked score stays minus infinity and a product of zero stays zero
@@ -375,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     auto runs_of = [&](uint32_t it, int sub) __attribute__((always_inline)) -> Runs {
         Runs x;
         x.bits = kAllRuns;
+        x.far = false;
         if constexpr (kRows == kExContiguous) {
             x.r[0] = x.r[1] = Run{factor_of(1.0f), 0.0f, 1.0f};
         } else {
@@ -384,6 +388,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             for (int a = 0; a < kLaneRuns; a++) {
                 const float4v r = s_run[at + (kFine ? 2 * a : a)];
                 x.bits |= r.w != 0.0f ? 1u << a : 0u;
+                if constexpr (kF8) x.far = x.far || r.w == 2.0f;
                 x.r[a] = kF8 ? Run{kQF32 ? factor_of(r.x) : r.x, r.y, r.z} : Run{factor_of(1.0f), 0.0f, 1.0f};
             }
             if constexpr (!kFine) x.bits = ex_uniform(x.bits);
@@ -436,10 +441,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         for (int r = 0; r < 16; r++) top = fmaxf(top, rounded_score(s[r], runs.r[r >> kRunShift].scale) + runs.r[r >> kRunShift].lvs);
         const LanePair both = half_wave_pair(top);
         const float m_new = fmaxf(m_ref, fmaxf(both.lo, both.hi));
-        const float alpha = fast_exp2(m_ref - m_new);
+        // (in two steps for the sum, which can be 2^100 times larger than the probabilities)
+        const float root = fast_exp2(0.5f * (m_ref - m_new)), alpha = root * root;
         m_ref = m_new;
         limit = fabsf(m_ref) < kFusedScores || m_ref == kExNegBig ? kProbLimit : 0.0f;
-        l_run *= alpha;
+        l_run = l_run * root * root;
 #pragma unroll
         for (int t = 0; t < kBlocks; t++)
 #pragma unroll
@@ -473,6 +479,18 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         float t = sum[0] + sum[1];
         if constexpr (kFine) t += sum[2] + sum[3];
         return t;
+    };
+    // The sum's weights of a sub-tile some of whose V scales are beyond 2^+-kPlainScales: probabilities times 1 / (V scale) would
+    // have vanished where the reference comes from a scale 2^102 larger (blocks of zeros, with the append's 2^-96,
+    // beside values of 1e4). Taken from the scores; the power of two is room towards the smallest float, and 2^100, the
+    // inverse of the smallest scale, times it is in range.
+    auto far_weights = [&](const float16v& s, const Runs& runs, float (&sum)[kLaneRuns]) __attribute__((always_inline)) {
+        float t = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) t += fast_exp2((rounded_score(s[r], runs.r[r >> kRunShift].scale) - m_ref) + 20.0f);
+        l_run += t * 0x1p-20f;
+#pragma unroll
+        for (int a = 0; a < kLaneRuns; a++) sum[a] = 0.0f;
     };
     auto accumulate = [&](uint32_t vbuf, int sub, const Probs& pr) __attribute__((always_inline)) {
         const uint16_t* sv = s_v0 + vbuf * kVTile + 32 * sub * kVPitch;
@@ -558,9 +576,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             p_out.lo[0] = ex_half8(uint4v{pl[0], pl[1], pl[2], pl[3]});
             p_out.lo[1] = ex_half8(uint4v{pl[4], pl[5], pl[6], pl[7]});
         }
-        if (__any(!(total_of(psum) < limit))) {  // rare: the reference has to move, redo the sub-tile
+        if (__any(!(total_of(psum) < limit) || runs_in.far)) {  // rare: the reference has to move, redo the sub-tile
             rebase(s_in, runs_in);
             probabilities_once(s_in, runs_in, p_out, psum);
+            if constexpr (kF8) {
+                if (__any(runs_in.far)) far_weights(s_in, runs_in, psum);
+            }
         }
 #pragma unroll
         for (int a = 0; a < kLaneRuns; a++) l_run += psum[a] * runs_in.r[a].inv;
@@ -804,15 +825,15 @@ __global__ void __launch_bounds__(256) kv_tiles_merge_kernel(KvParams p) {
         float m_new = mx;
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) m_new = fmaxf(m_new, s0 + i < p.n_splits ? m[i] : kExNegBig);
-        const float keep = fast_exp2(mx - m_new);
-        l *= keep;
+        const float keep_root = fast_exp2(0.5f * (mx - m_new)), keep = keep_root * keep_root;  // two steps as in rebase
+        l = l * keep_root * keep_root;
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e] *= keep;
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
             if (s0 + i >= p.n_splits) continue;
-            const float f = fast_exp2(m[i] - m_new);
-            l += ls[i] * f;
+            const float root = fast_exp2(0.5f * (m[i] - m_new)), f = root * root;
+            l += ls[i] * root * root;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 o[e] += a[i][e] * f;

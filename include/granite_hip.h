@@ -470,8 +470,8 @@ int granite_hip_matvec_q4k_batched(const void *x, int64_t x_stride, const void *
  * float scale for each (block, KV head) of K and of V, [num_blocks, num_kv_heads]: an element is
  * code * scale.  granite_hip_rope_append_q8 writes scales that are powers of two (a power of two
  * costs a floating-point code nothing, and a scale that grows later moves the codes of its block by
- * whole exponents, which is exact down to code 2^-6); the attention entry points take any positive
- * finite scale.
+ * whole exponents, which is exact down to code 2^-6); the attention entry points take any scale from 2^-96 to
+ * 2^120, the append's range, however far apart those of different blocks are.
  *
  * Attention with these forms:
  *   - a block-table entry outside [0, num_blocks) is never followed: its tokens count as not visible.
@@ -481,7 +481,8 @@ int granite_hip_matvec_q4k_batched(const void *x, int64_t x_stride, const void *
  *     a log-sum-exp of minus infinity, as does one all of whose scores are minus infinity;
  *   - K or V values of tokens that a query does not see never reach its result, also where they are
  *     NaN or infinite.
- * Sums and accumulators are float.  Probabilities enter the second product as a half and a half remainder,
+ * Sums and accumulators are float; a probability below 2^-126 of its row's largest counts as zero.
+ * Probabilities enter the second product as a half and a half remainder,
  * 22 bits; with half outputs and many rows as one half.  A row (token and head) of float queries is scaled by
  * a power of two and split into a half and a half remainder: an element of a row of any magnitude counts to
  * within 2^-23 of itself or 2^-40 of the row's largest, whichever is more. */

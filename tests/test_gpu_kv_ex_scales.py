@@ -79,6 +79,23 @@ def test_a_later_tokens_scale_does_not_count(gpu, name):
     check_run(gpu, cache.upload(), q, total - n, window, range(n - 1), tiles, F32, what=name)
 
 
+@pytest.mark.parametrize("other", [20, 60, 110])
+@pytest.mark.parametrize("name", [n for n in RUNS if RUNS[n][0] == F8E4M3])
+def test_blocks_of_zeros_keep_their_weight(gpu, name, other):
+    """Every other block's V is zero (its scale 2^-96, as the append leaves it), the rest have scales of 2^other: the zeros
+    count in the sums as any value does."""
+    cache, shape, start, window, some, tiles = run_cache(name)
+    cache.vs[:] = 2.0 ** other / 64
+    for block in range(0, -(-cache.lens[0] // cache.bs), 2):
+        b = cache.table[0, block]
+        cache.v[b * cache.bs:(b + 1) * cache.bs] = 0
+        cache.vs[b] = 2.0 ** -96
+    cache.upload()
+    for q_dtype in (np.float16, np.float32):
+        q = np.random.default_rng(2).standard_normal(shape).astype(q_dtype)
+        check_run(gpu, cache, q, start, window, some, tiles, F32, what=f"{name} 2^{other}")
+
+
 @pytest.mark.parametrize("name", [n for n in STEPS if STEPS[n][0] == F8E4M3])
 def test_both_ends_of_the_scales(gpu, name):
     for ks, vs, scale in ((2.0 ** -96, 2.0 ** -96, 2.0 ** 90), (2.0 ** 112, 2.0 ** 112, 2.0 ** -118)):
@@ -86,3 +103,13 @@ def test_both_ends_of_the_scales(gpu, name):
         cache.ks[:], cache.vs[:] = ks, vs
         q = np.random.default_rng(2).standard_normal(shape).astype(np.float16)
         check_step(gpu, cache.upload(), q, window, some, scale, f"{name} {ks}")
+
+
+@pytest.mark.parametrize("name", [n for n in RUNS if RUNS[n][0] == F8E4M3])
+def test_both_ends_of_the_scales_in_a_run(gpu, name):
+    for ks, vs, scale in ((2.0 ** -96, 2.0 ** -96, 2.0 ** 90), (2.0 ** 112, 2.0 ** 112, 2.0 ** -118)):
+        for q_dtype in (np.float16, np.float32):
+            cache, shape, start, window, some, tiles = run_cache(name)
+            cache.ks[:], cache.vs[:] = ks, vs
+            q = np.random.default_rng(2).standard_normal(shape).astype(q_dtype)
+            check_run(gpu, cache.upload(), q, start, window, some, tiles, F32, scale, f"{name} {ks}")
