@@ -108,13 +108,15 @@ __device__ __forceinline__ half8 as_half8(uint4v x) { return __builtin_bit_cast(
 __device__ __forceinline__ void dma_rows(uint32_t lds_addr, const void* sbase, uint32_t lane_off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
-                 : "s"(lds_addr), "v"(lane_off), "s"(sbase));
+                 : "s"(lds_addr), "v"(lane_off), "s"(sbase)
+                 : "m0");
 }
 // 64-bit address per lane:
 __device__ __forceinline__ void dma_lanes(uint32_t lds_addr, const void* addr) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
-                 : "s"(lds_addr), "v"(addr));
+                 : "s"(lds_addr), "v"(addr)
+                 : "m0");
 }
 template <int kCount>
 __device__ __forceinline__ void wait_transfers() {
