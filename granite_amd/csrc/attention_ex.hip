@@ -47,6 +47,7 @@ constexpr int kKBuffers = 3, kVBuffers = 3;
 constexpr uint32_t kPlan = 64;  // tiles whose rows and scales are worked out at a time
 constexpr float kProbLimit = 16384.0f;  // a row's probabilities of a sub-tile may sum to this much
 constexpr float kPlainScales = 48.0f;   // V scales within 2^-48 .. 2^48 take the sum's weights from the probabilities
+constexpr uint32_t kFarScale = 1u << 8;   // others
 constexpr float kFusedScores = 0x1p20f;  // references below this leave scores to a fused multiply-add
 
 template <int kD, int kRows>
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     uint16_t* const s_k0 = s_mem;
     uint16_t* const s_v0 = s_mem + kKBuffers * kKTile;
     // of run i of the workgroup's j-th tile, at (j mod 128) * kTileRuns + i: scale of the scores, log2 of the V scale, its inverse,
-    // 0 (no page of the pool's), 1 or 2 (a V scale beyond 2^+-kPlainScales)
+    // bits (the place of the run among those of a lane's 16 scores, where its page is one of the pool's; kFarScale)
     float4v* const s_run = reinterpret_cast<float4v*>(reinterpret_cast<unsigned char*>(s_mem) + S::kTileBytes);
     uint32_t* const s_special = reinterpret_cast<uint32_t*>(s_run + 2 * kPlan * kTileRuns);
 
@@ -270,8 +271,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             else info.x = kF8 && valid ? fmaxf(fmaxf(r.ks[f], 0.0f) * p.scale_log2, 0x1p-126f) : p.scale_log2;
             info.y = kF8 ? __builtin_amdgcn_logf(vs) : 0.0f;
             info.z = 1.0f / vs;
-            info.w = !valid ? 0.0f : fabsf(info.y) > kPlainScales ? 2.0f : 1.0f;
-            s_run[(half * kPlan + lane) * kTileRuns + (kFine ? 2 * wave + f : wave >> 1)] = info;
+            const uint32_t run = kFine ? 2 * wave + f : wave >> 1, place = kFine ? (run >> 1) & 3 : run & 1;
+            info.w = __uint_as_float(!valid ? 0u : (1u << place) | (fabsf(info.y) > kPlainScales ? kFarScale : 0u));
+            s_run[(half * kPlan + lane) * kTileRuns + run] = info;
         }
     };
     // a tile's planned rows: one value for the wave, or one for its first four keys and one for the others
@@ -367,8 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     };
     struct Runs {
         Run r[kLaneRuns];
-        uint32_t bits;  // of those whose page is one of the pool's
-        bool far;       // one has a V scale beyond 2^+-kPlainScales
+        uint32_t bits;  // of those whose page is one of the pool's; kFarScale
     };
     constexpr uint32_t kAllRuns = (1u << kLaneRuns) - 1;
     // positive and finite, so that a masked score stays minus infinity and a product of zero stays zero
@@ -378,7 +379,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     auto runs_of = [&](uint32_t it, int sub) __attribute__((always_inline)) -> Runs {
         Runs x;
         x.bits = kAllRuns;
-        x.far = false;
         if constexpr (kRows == kExContiguous) {
             x.r[0] = x.r[1] = Run{factor_of(1.0f), 0.0f, 1.0f};
         } else {
@@ -387,8 +387,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
 #pragma unroll
             for (int a = 0; a < kLaneRuns; a++) {
                 const float4v r = s_run[at + (kFine ? 2 * a : a)];
-                x.bits |= r.w != 0.0f ? 1u << a : 0u;
-                if constexpr (kF8) x.far = x.far || r.w == 2.0f;
+                x.bits |= __float_as_uint(r.w);
                 x.r[a] = kF8 ? Run{kQF32 ? factor_of(r.x) : r.x, r.y, r.z} : Run{factor_of(1.0f), 0.0f, 1.0f};
             }
             if constexpr (!kFine) x.bits = ex_uniform(x.bits);
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     };
     // keys of the sub-tile at key0 that the lane's row does not see become minus infinity
     auto apply_mask = [&](uint32_t key0, uint32_t bits, float16v& s) __attribute__((always_inline)) {
-        if (key0 + 32 <= every_hi && (key0 >= every_lo || key0 + 32 <= p.sinks) && (kFine ? __all(bits == kAllRuns) : bits == kAllRuns)) return;
+        if (key0 + 32 <= every_hi && (key0 >= every_lo || key0 + 32 <= p.sinks) && (kFine ? __all((bits & kAllRuns) == kAllRuns) : (bits & kAllRuns) == kAllRuns)) return;
         // what depends on the lane goes into three numbers, the rest is a constant per element; no short-circuit logic,
         // so that it stays compares and selects
         const int32_t base = int32_t(key0 + 4 * g), lo = int32_t(row_lo) - base, sink = int32_t(p.sinks) - base;
@@ -576,11 +575,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             p_out.lo[0] = ex_half8(uint4v{pl[0], pl[1], pl[2], pl[3]});
             p_out.lo[1] = ex_half8(uint4v{pl[4], pl[5], pl[6], pl[7]});
         }
-        if (__any(!(total_of(psum) < limit) || runs_in.far)) {  // rare: the reference has to move, redo the sub-tile
+        if (__any(!(total_of(psum) < limit) || (kF8 && (runs_in.bits & kFarScale)))) {  // rare: the reference has to move, redo the sub-tile
             rebase(s_in, runs_in);
             probabilities_once(s_in, runs_in, p_out, psum);
             if constexpr (kF8) {
-                if (__any(runs_in.far)) far_weights(s_in, runs_in, psum);
+                if (__any(runs_in.bits & kFarScale)) far_weights(s_in, runs_in, psum);
             }
         }
 #pragma unroll
