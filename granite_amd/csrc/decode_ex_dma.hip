@@ -442,10 +442,10 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
             for (int i = 0; i < 4; i++) {
                 const float d = s[sub][i] - m_new;
                 l_run += fast_exp2(d);
-                const float scaled = fast_exp2(d + shift) * f;
-                const _Float16 h = static_cast<_Float16>(scaled);
-                hi[4 * sub + i] = h;
-                rem[4 * sub + i] = static_cast<_Float16>(scaled - static_cast<float>(h));
+                _Float16 half, rest;
+                ex_split(fast_exp2(d + shift) * f, half, rest);
+                hi[4 * sub + i] = half;
+                rem[4 * sub + i] = rest;
             }
         }
         if (kMulti && masked) {

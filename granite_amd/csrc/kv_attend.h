@@ -95,6 +95,15 @@ __device__ __forceinline__ float ex_power(int e) { return __uint_as_float(uint32
 // A V scale as mantissa (0.5 <= . < 1) and exponent.
 __device__ __forceinline__ float ex_exponent(float vs) { return float(__builtin_amdgcn_frexp_expf(vs)); }
 __device__ __forceinline__ float ex_mantissa(float vs) { return __builtin_amdgcn_frexp_mantf(vs); }
+// A product as a half and the half remainder of it.  The product is pinned as the float it rounds to: where the compiler
+// may fuse it, it took the half of the exact product for the remainder and that of the rounded one for the operand, and where
+// the two lie either side of a tie the pair was half a step of a half, 2^-11, off.
+__device__ __forceinline__ void ex_split(float product, _Float16& half, _Float16& rest) {
+    asm volatile("" : "+v"(product));
+    half = static_cast<_Float16>(product);
+    rest = static_cast<_Float16>(product - static_cast<float>(half));
+}
+
 // What an accumulator relative to `bound` (log2, see Rows16) counts.
 __device__ __forceinline__ float ex_unit(float bound) { return __builtin_ldexpf(1.0f / kExBoost, int(fmaxf(ceilf(bound), -200.0f))); }
 
@@ -532,9 +541,10 @@ __device__ __forceinline__ void attend_tile(const KvParams& p, Tile<kF8, kRows, 
                 const float vs = of_token(rows.vs, sub, i);
                 scaled = fast_exp2(d + (ex_exponent(vs) - whole)) * (ex_mantissa(vs) * kExBoost);
             }
-            const _Float16 h = static_cast<_Float16>(scaled);
-            hi8[sub / 2][4 * (sub % 2) + i] = h;
-            lo8[sub / 2][4 * (sub % 2) + i] = static_cast<_Float16>(scaled - static_cast<float>(h));
+            _Float16 half, rest;
+            ex_split(scaled, half, rest);
+            hi8[sub / 2][4 * (sub % 2) + i] = half;
+            lo8[sub / 2][4 * (sub % 2) + i] = rest;
         }
 #pragma unroll
     for (int pair = 0; pair < T::kPairs; pair++)

@@ -113,3 +113,30 @@ def test_both_ends_of_the_scales_in_a_run(gpu, name):
             cache.ks[:], cache.vs[:] = ks, vs
             q = np.random.default_rng(2).standard_normal(shape).astype(q_dtype)
             check_run(gpu, cache.upload(), q, start, window, some, tiles, F32, scale, f"{name} {ks}")
+
+
+@pytest.mark.parametrize("bs,hq,hkv,d", [(16, 48, 3, 64), (20, 48, 1, 128), (8, 64, 4, 64), (1, 40, 8, 64), (48, 64, 2, 128)])
+def test_scales_of_any_value_in_a_step(gpu, bs, hq, hkv, d):
+    """Few keys a row, so that a single probability that is off shows."""
+    for q_dtype in (np.float16, np.float32):
+        cache = Cache(np.random.default_rng(hq), [*range(1, 25), 40, 80], bs, hkv, d, F8E4M3, scales="any", spread=3.0).upload()
+        q = np.random.default_rng(2).standard_normal((26, hq, d)).astype(q_dtype)
+        check_step(gpu, cache, q, (0, 0), range(26), what=f"bs={bs} {q_dtype.__name__}")
+
+
+@pytest.mark.parametrize("name", [n for n in STEPS if STEPS[n][0] == F8E4M3])
+def test_scales_of_any_value_behind_long_contexts(gpu, name):
+    cache, shape, window, some = step_cache(name)
+    cache.vs *= np.random.default_rng(3).uniform(1, 1.9, cache.vs.shape).astype(np.float32)
+    cache.ks *= np.random.default_rng(4).uniform(1, 1.9, cache.ks.shape).astype(np.float32)
+    q = (np.random.default_rng(2).standard_normal(shape) * 12).astype(np.float16)  # a few keys carry each row
+    check_step(gpu, cache.upload(), q, window, some, what=name)
+
+
+@pytest.mark.parametrize("n,start,bs,hq,hkv,d,tiles", [(30, 5, 32, 64, 2, 64, False), (60, 11, 5, 34, 2, 64, False), (12, 19, 16, 64, 2, 128, False),
+                                                       (420, 0, 16, 96, 1, 64, True), (420, 3, 20, 96, 1, 128, True)])
+def test_scales_of_any_value_in_a_run(gpu, n, start, bs, hq, hkv, d, tiles):
+    for q_dtype in (np.float16, np.float32):
+        cache = Cache(np.random.default_rng(hq), [start + n], bs, hkv, d, F8E4M3, scales="any", spread=3.0).upload()
+        q = np.random.default_rng(2).standard_normal((n, hq, d)).astype(q_dtype)
+        check_run(gpu, cache, q, start, (0, 0), range(0, min(n, 60), 2), tiles, F32, what=f"n={n} {q_dtype.__name__}")
