@@ -19,17 +19,20 @@
 //   log2 domain.  V's enters the exponent: with x = score + log2(v scale) the probabilities p' = exp2(x - ref)
 //   carry it, the second product takes the codes, and the sum l takes each run's p' times 1 / (v scale).  The
 //   reference follows x, so a large or small V scale never pushes p' out of the range of a half.  Cost per sub-tile:
-//   two subtractions and one more multiply-add than without scales.
+//   two subtractions and one more multiply-add than without scales.  Where a scale is beyond 2^+-48, p' may have vanished
+//   that the sum should count; such a sub-tile's part of l is worked out from the scores (rare).
 // * Tiles are visited by the list of kv_visible.h: those of the sinks, then those of the window.
 //
 // Measured (half Q and results): 512 queries of 64 heads over 8 KV heads of 128 behind 32768 keys 535 to 572 us a call, 1.0 PFLOP/s
-// (a large half matrix product reaches 1.17); 4096 queries of 32 heads of 64 through a window of 4096 198 us, 0.69 PFLOP/s;
+// (a large half matrix product reaches 1.17); 4096 queries of 32 heads of 64 through a window of 4096 196 us, 0.70 PFLOP/s;
 // 2048 queries of 32 heads of 128 through a window of 512 31 us.  What bounds it: a tile is 64 MFMAs on a SIMD, 2048 cycles,
 // and some 370 vector instructions beside them (softmax, conversions of codes and probabilities), 6 a MFMA at head size
 // 128 and 11 at 64; the matrix cores are busy 45 % (27 %) of the time.
 //
-// Probabilities are rounded to half; with float outputs (kPrecise) they are a half and a half remainder and the
-// second product runs twice.  Sums and accumulators are float.
+// Probabilities are rounded to half: against float64 a half result is then 2.9e-4 off (root mean square, relative) where
+// its own rounding alone would leave 2.1e-4, and a second product for the remainders costs a third more.  That is what float
+// outputs get (kPrecise): a half and a half remainder, the second product twice (512 queries behind 32768 keys 748 us where half
+// outputs take 553); float queries are two halves as well, the first product twice (897 us).  Sums and accumulators are float.
 //
 // V of keys that no row of the workgroup sees is stored as zeros, since 0 * NaN is NaN.  In tiles that only
 // some rows see, infinities and NaNs of V are stored as zeros as well, and where there were any they are added

@@ -20,7 +20,7 @@
 // compiler waits for would wait for all transfers in flight.
 //
 // Measured (group of 4 or 8 heads over 8 KV heads of 128, half Q, whole call with the merge): 64 sequences of 256 to 8192 tokens
-// 97 us for 556 MB, 5.7 TB/s; 2 of 131072 92 us for 515 MB, 5.6 TB/s.  Without the arithmetic (timing only) the kernel takes
+// 98 us for 556 MB, 5.7 TB/s; 2 of 131072 92 us for 515 MB, 5.6 TB/s.  Without the arithmetic (timing only) the kernel takes
 // as long: what bounds it is the pattern of memory accesses, 7 us until the first tiles have come and waves that end
 // 15 to 28 us apart.
 #include "common.h"

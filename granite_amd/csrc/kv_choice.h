@@ -5,8 +5,9 @@
 // up, and every 16 rows read their keys again.  The persistent kernel has 16 a wave, a fixed number of waves and no tail.  The
 // tiles kernel has 256 a workgroup and runs at the rate of the matrix cores, behind a long prologue.  The constants are
 // fits to 160 calls drawn over 2 to 1500 queries, 1 to 16 KV heads, contexts up to 33000 and windows from 1 on, each timed on
-// all three (following the estimates costs 1.7 % over the best of the three on 100 other calls, a rule on the number of
-// rows alone 34 %), and to 150 decode steps of 1 to 64 sequences (0.7 %; by the length of the context alone 4.5 %).
+// all three, and to 150 decode steps of 1 to 64 sequences on the two that take them.  What following the estimates costs over
+// the best kernel of each call: 2.3 % over those 160 (the worst 1.6 times), 1.7 % over 100 others (1.3 times), 0.8 % over the steps
+// (1.4 times).
 #pragma once
 
 #include <stdint.h>

@@ -20,8 +20,10 @@
 //   * Q: a thread per eight elements of a token's row in one or kQHeads heads, cos and sin loaded once for all.
 //
 // Measured (32 query heads over 8 KV heads of 128): 8187 tokens, half in and float Q out, 59.9 us a call for 256 MB, 4.3 TB/s,
-// where a large copy reaches 4.9 (66 us with one head a thread and a wave a block); 64 tokens of 64 sequences 3.2 us of
-// kernel in a call of 7.8 us: the launch; 512 tokens (64 heads) 8.4 us a call, 3.7 TB/s.
+// where a large copy reaches 4.9 (66 us with one head a thread and a wave a block); 64 tokens of 64 sequences, each the first of its
+// block, 3.2 us of kernel in a call of 7.8 us: the launch; 512 tokens (64 heads) 8.5 us a call, 3.7 TB/s.  A scale that grows late
+// in a block costs a step more: a wave walks the rows in front one after the other.  The kernel on its own, at the clocks of a few
+// calls: 5.5 us for tokens that start a block or leave its scale, 7.9 where every scale grows at row 15 of 16, 32 at row 127 of 128.
 #include <algorithm>
 #include <cmath>
 
