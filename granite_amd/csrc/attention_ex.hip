@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         // (in two steps for the sum, which can be 2^100 times larger than the probabilities)
         const float root = fast_exp2(0.5f * (m_ref - m_new)), alpha = root * root;
         m_ref = m_new;
-        limit = fabsf(m_ref) < kFusedScores || m_ref == kExNegBig ? kProbLimit : 0.0f;
+        if (!(fabsf(m_ref) < kFusedScores) && m_ref != kExNegBig) limit = 0.0f;
         l_run = l_run * root * root;
 #pragma unroll
         for (int t = 0; t < kBlocks; t++)
@@ -482,10 +482,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
         if constexpr (kFine) t += sum[2] + sum[3];
         return t;
     };
-    // The sum's weights of a sub-tile some of whose V scales are beyond 2^+-kPlainScales: probabilities times 1 / (V scale) would
-    // have vanished where the reference comes from a scale 2^102 larger (blocks of zeros, with the append's 2^-96,
-    // beside values of 1e4). Taken from the scores; the power of two is room towards the smallest float, and 2^100, the
-    // inverse of the smallest scale, times it is in range.
+    // The sum's weights of a sub-tile some of whose V scales are beyond 2^+-kPlainScales, and of every one behind a scale above
+    // 2^kPlainScales, from which the reference may come: probabilities times 1 / (V scale) would have vanished where the
+    // reference comes from a scale 2^102 larger (blocks of zeros, with the append's 2^-96, beside values of 1e4).  Taken from
+    // the scores; the power of two is room towards the smallest float, and 2^100, the inverse of the smallest scale, times it
+    // is in range.
     auto far_weights = [&](const float16v& s, const Runs& runs, float (&sum)[kLaneRuns]) __attribute__((always_inline)) {
         float t = 0.0f;
 #pragma unroll
@@ -582,7 +583,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
             rebase(s_in, runs_in);
             probabilities_once(s_in, runs_in, p_out, psum);
             if constexpr (kF8) {
-                if (__any(runs_in.bits & kFarScale)) far_weights(s_in, runs_in, psum);
+                bool high = false;
+#pragma unroll
+                for (int a = 0; a < kLaneRuns; a++) high = high || runs_in.r[a].lvs > kPlainScales;
+                if (__any(high)) limit = 0.0f;  // this way from here on
+                if (__any((runs_in.bits & kFarScale) || limit == 0.0f)) far_weights(s_in, runs_in, psum);
             }
         }
 #pragma unroll

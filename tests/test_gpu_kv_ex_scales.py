@@ -140,3 +140,24 @@ def test_scales_of_any_value_in_a_run(gpu, n, start, bs, hq, hkv, d, tiles):
         cache = Cache(np.random.default_rng(hq), [start + n], bs, hkv, d, F8E4M3, scales="any", spread=3.0).upload()
         q = np.random.default_rng(2).standard_normal((n, hq, d)).astype(q_dtype)
         check_run(gpu, cache, q, start, (0, 0), range(0, min(n, 60), 2), tiles, F32, what=f"n={n} {q_dtype.__name__}")
+
+
+@pytest.mark.parametrize("name", [n for n in RUNS if RUNS[n][0] == F8E4M3])
+def test_scales_all_over_the_range_in_a_run(gpu, name):
+    """Every block's V scale anywhere from 2^-88 to 2^95, so that the largest come late for some rows and early for others."""
+    for seed, q_dtype in ((1, np.float16), (2, np.float32), (3, np.float16)):
+        cache, shape, start, window, some, tiles = run_cache(name)
+        rng = np.random.default_rng(seed)
+        cache.vs = (cache.vs * 2.0 ** rng.integers(-80, 100, cache.vs.shape)).astype(np.float32)
+        q = (rng.standard_normal(shape) * rng.choice([0.3, 3.0])).astype(q_dtype)
+        check_run(gpu, cache.upload(), q, start, window, some, tiles, F32, what=f"{name} {seed}")
+
+
+@pytest.mark.parametrize("name", [n for n in STEPS if STEPS[n][0] == F8E4M3])
+def test_scales_all_over_the_range_in_a_step(gpu, name):
+    for seed, q_dtype in ((1, np.float16), (2, np.float32)):
+        cache, shape, window, some = step_cache(name)
+        rng = np.random.default_rng(seed)
+        cache.vs = (cache.vs * 2.0 ** rng.integers(-80, 100, cache.vs.shape)).astype(np.float32)
+        q = (rng.standard_normal(shape) * rng.choice([0.3, 3.0])).astype(q_dtype)
+        check_step(gpu, cache.upload(), q, window, some, what=f"{name} {seed}")
