@@ -480,10 +480,12 @@ int granite_hip_matvec_q4k_batched(const void *x, int64_t x_stride, const void *
  *   - a query that sees no key (its window lies behind the cache, every page invalid) gets zeros and
  *     a log-sum-exp of minus infinity, as does one all of whose scores are minus infinity;
  *   - K or V values of tokens that a query does not see never reach its result, also where they are
- *     NaN or infinite.
+ *     NaN or infinite.  Those of tokens that it sees do, as the formula has them, but for an infinity in K
+ *     of a half cache under a float query, which makes the result NaN whatever its sign (the query is two
+ *     halves there, see below).
  * Sums and accumulators are float; a probability below 2^-126 of its row's largest counts as zero.
- * Probabilities enter the second product as a half and a half remainder,
- * 22 bits; with half outputs and many rows as one half.  A row (token and head) of float queries is scaled by
+ * Probabilities enter the second product as a half and a half remainder, to within 2^-22 of themselves or 2^-25
+ * of the row's largest; with half outputs and many rows as one half.  A row (token and head) of float queries is scaled by
  * a power of two and split into a half and a half remainder: an element of a row of any magnitude counts to
  * within 2^-23 of itself or 2^-40 of the row's largest, whichever is more. */
 typedef struct granite_hip_kv_form {

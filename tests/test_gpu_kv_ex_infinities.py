@@ -61,3 +61,28 @@ def test_scale_pointers_of_a_half_cache_mean_nothing(gpu, bs, batch, hq, hkv, d)
     rows = kv_ex_calls.prefill(gpu, cache, np.repeat(q[:1], 5, 0), 2995, F32, 2500, 4)[0]
     same = kv_ex_calls.prefill(gpu, cache, np.repeat(q[:1], 5, 0), 2995, F32, 2500, 4, k_scale=scales, v_scale=scales)[0]
     assert np.array_equal(rows, same)
+
+
+@pytest.mark.parametrize("bs,n,hq,hkv,d", [(16, 1, 4, 2, 128), (20, 5, 4, 2, 64), (16, 420, 96, 1, 64), (0, 300, 32, 1, 128)])
+def test_infinite_keys_under_half_queries(gpu, bs, n, hq, hkv, d):
+    """A key whose score is minus infinity has no weight; with a score of plus infinity a row is NaN."""
+    length, window, token = 700 + n, 600, 690
+    cache = Cache(np.random.default_rng(n), [length], bs, hkv, d, F16)
+    row = cache.table[0, token // bs] * bs + token % bs if bs else token
+    cache.k[(row, 0, 7) if bs else (0, row, 7)] = -np.inf
+    q = np.random.default_rng(n + 1).standard_normal((n, hq, d)).astype(np.float16)
+    got, lse = kv_ex_calls.prefill(gpu, cache.upload(), q, length - n, F32, window)
+    group = hq // hkv
+    position = length - n + np.arange(n)[:, None]
+    sees = (token <= position) & (token > position - window) & (np.arange(hq)[None] < group)
+    assert sees.any()
+    above = sees & (q[..., 7] < 0)
+    assert np.array_equal(np.isnan(got).all(-1), above) and np.array_equal(np.isnan(got).any(-1), above) and np.array_equal(np.isnan(lse), above)
+    # the others: as with a finite key of no weight there
+    cache.k[(row, 0, 7) if bs else (0, row, 7)] = -60000.0
+    inf, inf_lse = got[sees & ~above], lse[sees & ~above]
+    got, lse = kv_ex_calls.prefill(gpu, cache.upload(), q, length - n, F32, window)
+    with_weight = sees & ~above & (q[..., 7] > 0.02)  # -60000 * 0.02 / sqrt(d): more than 100 below the other scores
+    pick = with_weight[sees & ~above]
+    np.testing.assert_allclose(inf[pick], got[with_weight], rtol=0, atol=1e-6)
+    np.testing.assert_allclose(inf_lse[pick], lse[with_weight], rtol=0, atol=1e-6)
