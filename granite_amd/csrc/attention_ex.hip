@@ -146,41 +146,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_tiles_kernel(KvParams p) {
     float q_unit = p.scale_log2;  // kQF32: of a product with the row as loaded in the log2 domain, the K scale apart; positive
     {
         const int64_t off = int64_t(query) * p.q_tok + int64_t(head) * p.q_head + 8 * g;
-        if constexpr (kQF32) {  // as Rows16::load_q
-            const float* const qr = static_cast<const float*>(p.q) + off;
-            float x[kSteps][8];
-#pragma unroll
-            for (int s = 0; s < kSteps; s++) {
-                const float* qp = qr + 16 * s;
-                const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[s][i] = x0[i];
-                    x[s][4 + i] = x1[i];
-                }
-            }
-            float top = 0.0f;
-#pragma unroll
-            for (int s = 0; s < kSteps; s++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[s][i]));
-            const LanePair both = half_wave_pair(top);
-            const int shift = ex_q_shift(fmaxf(both.lo, both.hi));
-            const float power = ex_power(shift) * p.q_sign;
-            q_unit = p.scale_log2 * ex_power(-shift);
-#pragma unroll
-            for (int s = 0; s < kSteps; s++) {
-                half8 hi, lo;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float xs = x[s][i] * power;
-                    const _Float16 h = static_cast<_Float16>(xs);
-                    hi[i] = h;
-                    lo[i] = static_cast<_Float16>(xs - static_cast<float>(h));
-                }
-                bq[s] = hi;
-                bq_lo[s] = lo;
-            }
+        if constexpr (kQF32) {
+            auto both_lanes = [](float v) {
+                const LanePair both = half_wave_pair(v);
+                return fmaxf(both.lo, both.hi);
+            };
+            q_unit = p.scale_log2 * ex_load_floats<kSteps>(static_cast<const float*>(p.q) + off, [](int s) { return 16 * s; }, both_lanes, p.q_sign, true, bq, bq_lo);
         } else {
 #pragma unroll
             for (int s = 0; s < kSteps; s++)

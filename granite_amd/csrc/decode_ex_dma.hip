@@ -285,40 +285,8 @@ __global__ void __launch_bounds__(kWaves* kWave, 2) kv_dma_kernel(KvParams p) {
             row_lo = all_lo = window_begin(u.len - 1, p.window);
         }
         auto d_of = [&](int s) __attribute__((always_inline)) { return 64 * (s / 2) + 16 * g + 8 * (s % 2); };
-        if constexpr (kQF32) {  // as Rows16::load_q
-            const float* const qr = static_cast<const float*>(p.q) + at;
-            float x[kSteps][8];
-#pragma unroll
-            for (int s = 0; s < kSteps; s++) {
-                const float* qp = qr + d_of(s);
-                const float4v x0 = *reinterpret_cast<const float4v*>(qp), x1 = *reinterpret_cast<const float4v*>(qp + 4);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[s][i] = x0[i];
-                    x[s][4 + i] = x1[i];
-                }
-            }
-            float top = 0.0f;
-#pragma unroll
-            for (int s = 0; s < kSteps; s++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[s][i]));
-            const int shift = ex_q_shift(max_over_groups(top));
-            const float power = ex_power(shift);
-            q_unit = p.scale_log2 * ex_power(-shift);
-#pragma unroll
-            for (int s = 0; s < kSteps; s++) {
-                half8 hi, lo;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float xv = live ? x[s][i] * power : 0.0f;
-                    const _Float16 h = static_cast<_Float16>(xv);
-                    hi[i] = h;
-                    lo[i] = static_cast<_Float16>(xv - static_cast<float>(h));
-                }
-                bq[s] = hi;
-                bq_lo[s] = lo;
-            }
+        if constexpr (kQF32) {
+            q_unit = p.scale_log2 * ex_load_floats<kSteps>(static_cast<const float*>(p.q) + at, d_of, [](float v) { return max_over_groups(v); }, 1.0f, live, bq, bq_lo);
         } else {
 #pragma unroll
             for (int s = 0; s < kSteps; s++) {
